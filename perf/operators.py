@@ -217,7 +217,8 @@ def _rows(s, T):
 def _power(amax, m_top, e_top):
     """The smallest power of two whose product with the largest code holds amax."""
     m, e = torch.frexp(amax)
-    return torch.ldexp(torch.ones_like(amax), (e - e_top + (m > m_top)).clamp(-126, 120))
+    e = torch.where(amax == 0, torch.full_like(e, -126), e - e_top + (m > m_top))
+    return torch.ldexp(torch.ones_like(amax), e.clamp(-126, 120))
 
 
 def _round(x, codes_t, top):
