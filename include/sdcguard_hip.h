@@ -438,6 +438,48 @@ int sdc_attn_check_noalloc(int dtype, const void* q, int64_t sqt, int64_t sqh, c
                            float* capq, float* capo, int64_t capw, void* capkv, int32_t* capkvm, int64_t caprows,
                            int samples, int has_write, int keep_kv, float* scores_out, hipStream_t stream);
 
+/* ---- rotary positions (no counterpart in the reference) ------------------------------------------------------
+ * y (T, H, D) = x with the pairs of each head's first `rot` elements rotated by the token's position, the rest copied:
+ * pair i, (i, i + rot/2) or (2 i, 2 i + 1) with interleaved != 0, becomes (a c - b s, b c + a s), c = mscale cos,
+ * s = mscale sin of 2 pi position turns[i]; inverse != 0: of the negative angle (the gradient of the forward call).
+ *   dtype 0 = bf16, 1 = fp16, 4 = fp32; element strides; y may be x.  positions (T): int32 or int64 (pos_bytes 4 or 8).
+ *   turns (rot/2) float64: turns a pair makes per position.  rot <= 2048. */
+int sdc_rope(int dtype, const void* x, int64_t sxt, int64_t sxh, int64_t sxd, void* y, int64_t syt, int64_t syh,
+             int64_t syd, int64_t T, int64_t H, int64_t D, const void* positions, int pos_bytes, const double* turns,
+             int64_t rot, int interleaved, double mscale, int inverse, hipStream_t stream);
+
+/* ---- appending to a paged cache, quantized, with the rotation on the way (no counterpart in the reference) ------
+ * key, val (T, Hkv, D) of dtype 0 = bf16 or 1 = fp16 into the slots that qsl, seq_lens and bt (as in sdc_attn_check)
+ * give the step's tokens.
+ *   cache: 0 = e4m3 codes, 1 = int8 codes, 2 = dtype itself (scales NULL).  kv (NB, Hkv, N, 2D): element strides
+ *     (cb, ch, cn), keys then values, last dimension contiguous.  scales (NB, Hkv, 2) fp32: element strides (sb, sh).
+ *   A page's scale: the smallest power of two that holds the largest finite |x| appended since its slot 0 was last
+ *     written; where it grows, the page's other slots are rescaled to it.  Requests must not share pages they write.
+ *   turns (rot/2), interleaved, mscale: as sdc_rope (rot 0: no rotation); positions (T) or NULL (the tokens' own).
+ *   q (T, Hq, D), or NULL: rotated into q_out (which may be q); rows past qsl[R] become zeros. */
+int sdc_kv_append(int dtype, int cache, const void* key, int64_t skt, int64_t skh, int64_t skd, const void* val,
+                  int64_t svt, int64_t svh, int64_t svd, int64_t T, int64_t Hkv, int64_t D, void* kv, int64_t cb,
+                  int64_t ch, int64_t cn, int64_t NB, int64_t N, float* scales, int64_t sb, int64_t sh,
+                  const int32_t* qsl, const int32_t* seq_lens, int64_t R, const int32_t* bt, int64_t sbt, int64_t W,
+                  const void* positions, int pos_bytes, const double* turns, int64_t rot, int interleaved,
+                  double mscale, const void* q, int64_t sqt, int64_t sqh, int64_t sqd, void* q_out, int64_t sot,
+                  int64_t soh, int64_t sod, int64_t Hq, hipStream_t stream);
+
+/* ---- attention over a paged cache of 8-bit codes (no counterpart in the reference) --------------------------------
+ * o (T, Hq, D) = softmax(scale q . k) v over the keys each query sees (causal; the last `window` of them, 0: all),
+ * lse (T, Hq; token stride slt; may be NULL) = the natural logarithm of the sum of exp(scale q . k).
+ *   dtype 0 = bf16, 1 = fp16 (q and o); cache 0 = e4m3, 1 = int8; kv, scales, qsl, seq_lens, bt as sdc_kv_append.
+ *   max_len: no sequence is longer (keys past it are not read); at most W * N.  D <= 256, Hq a multiple of Hkv.
+ *   A query without keys, and rows past qsl[R]: zeros and -inf.  A key whose page lies outside the cache is NaN.
+ *   workspace: sdc_kv_attend_workspace(T, R, Hq, Hkv, D, max_len) bytes (may be NULL where that is 0). */
+int64_t sdc_kv_attend_workspace(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
+int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, int64_t sqh, int64_t sqd, void* o, int64_t sot,
+                  int64_t soh, int64_t sod, float* lse, int64_t slt, int64_t T, int64_t Hq, int64_t D, const void* kv,
+                  int64_t cb, int64_t ch, int64_t cn, int64_t NB, int64_t Hkv, int64_t N, const float* scales,
+                  int64_t sb, int64_t sh, const int32_t* qsl, const int32_t* seq_lens, int64_t R, const int32_t* bt,
+                  int64_t sbt, int64_t W, float scale, int64_t window, int64_t max_len, void* workspace,
+                  int64_t workspace_bytes, hipStream_t stream);
+
 /* ---- per-kernel timing (no counterpart in the reference; for benchmarks) ------------------------------------
  * With profiling on, every kernel launch is bracketed by two HIP events on its stream; sdc_profile_read waits for
  * them and sums the durations of one kernel: "expected_gemm" (serving GEMM), "serve_fused", "serve_sums",
@@ -446,7 +488,7 @@ int sdc_attn_check_noalloc(int dtype, const void* q, int64_t sqt, int64_t sqh, c
  * "quant_score_i8", "quant_score_fp8", "quant_consts", "fingerprint3", "fingerprint2", "kv_fingerprint", "attn_check", "acc_bsums",
  * "acc_gemm", "acc_score" (sdc_matmul_check_acc, sdc_matmul_check_acc_stats),
  * "fused_pack", "fused_side", "fused_mm", "fused_mm_checked" (sdc_fused_mm, sdc_fused_mm_checked), "fp8q_amax",
- * "fp8q_judge" (sdc_fp8_quant_check), "moe_up", "moe_act", "moe_down", "moe_compare" (sdc_moe_check), "route_check" (sdc_route_check). */
+ * "fp8q_judge" (sdc_fp8_quant_check), "moe_up", "moe_act", "moe_down", "moe_compare" (sdc_moe_check), "route_check" (sdc_route_check), "rope", "kv_append", "kv_attend". */
 int sdc_profile_enable(int on);
 int sdc_profile_reset(void);
 int sdc_profile_read(const char* name, double* total_ms, int64_t* launches);

@@ -24,7 +24,7 @@ DT_BF16, DT_FP16 = 0, 1
 _lock = threading.Lock()
 _lib = [None]
 
-P, I64, I32, F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+P, I64, I32, F32, F64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_double
 
 # name -> (restype, argtypes), in include/sdcguard_hip.h order
 SIGNATURES = {
@@ -89,6 +89,13 @@ SIGNATURES = {
                                      I64, F32, I64, F32, P, P, P, I64, P, P, I64, I32, I32, I32, P, P]),
     "sdc_quant_constants_workspace": (I64, [I32, I64, I64]),
     "sdc_quant_constants": (I32, [I32, P, I64, I64, I64, I64, I64, P, P, P, P, P, P, I64, P]),
+    "sdc_rope": (I32, [I32, P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, P, I32, P, I64, I32, F64, I32, P]),
+    "sdc_kv_append": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, P, I64, I64, I64, I64, I64, P,
+                            I64, I64, P, P, I64, P, I64, I64, P, I32, P, I64, I32, F64, P, I64, I64, I64, P, I64, I64,
+                            I64, I64, P]),
+    "sdc_kv_attend_workspace": (I64, [I64, I64, I64, I64, I64, I64]),
+    "sdc_kv_attend": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64, P, I64, I64, I64, I64,
+                            I64, I64, P, I64, I64, P, P, I64, P, I64, I64, F32, I64, I64, P, I64, P]),
     "sdc_mfma_layout_selftest": (I32, [P, P, P, P]),
     "sdc_last_error": (ctypes.c_char_p, []),
     "sdc_profile_enable": (I32, [I32]),

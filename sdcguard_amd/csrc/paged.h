@@ -1,0 +1,52 @@
+// What the append to a paged cache and the attention over it share: the step's metadata, and which request a query
+// token or a work item belongs to.
+#pragma once
+#include "common.h"
+
+// Element kinds of a cache.
+enum SdcCache { SDC_CACHE_E4M3 = 0, SDC_CACHE_I8 = 1, SDC_CACHE_16 = 2 };
+
+struct PagedStep {
+  const int32_t* qsl;          // (R + 1): where each request's query tokens start, non-decreasing
+  const int32_t* lens;         // (R): tokens of the request, this step's included
+  const int32_t* bt;           // (R, W): the page of each run of N positions
+  int64_t sbt, W, NB, T;
+  int R, N;
+};
+
+// One request: its query tokens q0 .. q1 - 1 are its last positions, up to len - 1 (position of token t:
+// t - q1 + len; a length shorter than the query leaves the first tokens without one).
+struct Request {
+  int r;
+  int64_t q0, q1, len;
+};
+
+// The last r in 0 .. R with qsl[r] / B + C r <= j, by the whole wave (all lanes active, j uniform), and -1 if there is
+// none; R stands for the tokens past the last request (the padding of a captured step).  Work items of up to B tokens each are numbered so that no scan over the requests is needed: request r's
+// items start at qsl[r] / B + C r.  With C = 1 that leaves room for items of B tokens from the request's first on, with
+// C = 2 for items that begin at positions divisible by B.  Every lane reads its requests' starts at once.
+__device__ __forceinline__ int sdc_request_of(const PagedStep& s, int64_t j, int B, int C) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int b = 0; b <= s.R; b += 64) {
+    const int i = b + lane;
+    const bool le = i <= s.R && (int64_t)((uint32_t)s.qsl[i] / (uint32_t)B) + (int64_t)C * i <= j;
+    const int c = __popcll(__ballot(le));
+    n += c;
+    if (c < 64) break;
+  }
+  return n - 1;
+}
+__device__ __forceinline__ Request sdc_request(const PagedStep& s, int r) {
+  Request q;
+  q.r = r;
+  q.q0 = min(max((int64_t)s.qsl[r], (int64_t)0), s.T);
+  if (r >= s.R) {
+    q.q1 = s.T;
+    q.len = 0;
+    return q;
+  }
+  q.q1 = min(max((int64_t)s.qsl[r + 1], q.q0), s.T);
+  q.len = max(s.lens[r], 0);
+  return q;
+}
