@@ -93,7 +93,7 @@ SIGNATURES = {
     "sdc_kv_append": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, I64, I64, I64, I64, P, I64, I64, I64, I64, I64, P,
                             I64, I64, P, P, I64, P, I64, I64, P, I32, P, I64, I32, F64, P, I64, I64, I64, P, I64, I64,
                             I64, I64, P]),
-    "sdc_kv_attend_workspace": (I64, [I64, I64, I64, I64, I64, I64]),
+    "sdc_kv_attend_workspace": (I64, [I64, I64, I64, I64, I64, I64, I64, I64]),
     "sdc_kv_attend": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64, P, I64, I64, I64, I64,
                             I64, I64, P, I64, I64, P, P, I64, P, I64, I64, F32, I64, I64, P, I64, P]),
     "sdc_mfma_layout_selftest": (I32, [P, P, P, P]),

@@ -150,7 +150,7 @@ def kv_attend(q: torch.Tensor, kv: torch.Tensor, scales: torch.Tensor, qsl: torc
         raise ValueError("max_seq_len must not be negative")
     L = _lib.lib()
     with torch.cuda.device(dev):
-        need = L.sdc_kv_attend_workspace(T, R, Hq, Hkv, D, most)
+        need = L.sdc_kv_attend_workspace(T, R, Hq, Hkv, D, N, most, int(window))
         ws = _lib.workspace(dev, need) if need else None
         rc = L.sdc_kv_attend(
             dt, code, q.data_ptr(), *q.stride(), out.data_ptr(), *out.stride(), _lib.ptr(lse), Hq, T, Hq, D,
