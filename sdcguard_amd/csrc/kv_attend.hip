@@ -4,9 +4,11 @@
 // lse = max s + log sum p.  A query that sees no key gets zeros and lse = -inf; a key in a page outside the cache
 // counts as NaN.
 //
-// The path for any head size and alignment: a wave per (query token, head), a key per lane for the products, then the
-// head's elements over the lanes for the sum of the values.
+// Three kernels.  kv_attend_rows: tiles of 16 query rows, for decode steps (HBM bound).  kv_attend_tiles: tiles of 256
+// query rows, for chunks of a prompt (bound by the matrix cores and the softmax between them).  kv_attend_any: any head
+// size and alignment.  A part of a tile's keys is one workgroup's; kv_attend_join joins the parts in their order.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "paged.h"
@@ -31,11 +33,16 @@ struct AttendArgs {
   int Hq, Hkv, G, D, fp16;
 };
 
-// The work of the tiled kernels: tiles of TB query tokens x GB heads of one kv head, whose keys are cut into at most S
-// parts of C keys, one part a workgroup.  part: (tile, part) records of ROWS (maximum, sum) pairs and ROWS x D sums.
+// The work of a tiled kernel: tiles of TB query tokens x GB heads of one kv head (at most `rows` query rows), whose keys
+// are cut into at most S parts, one part a workgroup.  A call with chunks runs both kernels: requests of up to `few`
+// tokens go to kv_attend_rows, the others, and the padding, to kv_attend_tiles.
+// part: (tile, part) records of `rows` (maximum, sum) pairs and rows x D sums.
 struct Split {
   int64_t tiles;
-  int TB, GB, NHB, C, S;
+  int TB, GB, NHB, S, rows;
+  int C;                                       // keys of a part at least (a multiple of 128)
+  int slots;                                   // tiles numbered by request, so many each (0: by their tokens)
+  int few;                                     // requests of up to so many tokens are left out (0: none)
   uint32_t div;                                // ceil(2^32 / N), to divide by N
   float* part;
 };
@@ -160,24 +167,41 @@ struct Tile {
   int r, hk, hb, ntok;                         // request (R: padding), kv head, block of GB heads, tokens
   int64_t tok0, p0;                            // first token and its position
   int64_t klo, khi, c0;                        // keys that some row sees, and where the parts are counted from
-  int nsp;                                     // parts with keys
+  int nsp, C;                                  // parts with keys, and their keys
 };
-__device__ __forceinline__ bool find_tile(const AttendArgs& a, const Split& sp, int id, Tile& t) {
-  t.hb = id % sp.NHB;
-  id /= sp.NHB;
-  t.hk = id % a.Hkv;
-  id /= a.Hkv;
-  t.r = sdc_request_of(a.st, id, sp.TB, 1);
-  if (t.r < 0) return false;
-  const Request rq = sdc_request(a.st, t.r);
-  t.tok0 = rq.q0 + (id - ((int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r)) * sp.TB;
-  if (t.tok0 < rq.q0 || t.tok0 >= rq.q1) return false;
+// the keys of a tile whose first token is given
+__device__ __forceinline__ void find_keys(const AttendArgs& a, const Split& sp, const Request& rq, Tile& t) {
   t.ntok = (int)min((int64_t)sp.TB, rq.q1 - t.tok0);
   t.p0 = t.r < a.st.R ? t.tok0 - rq.q1 + rq.len : -(int64_t)sp.TB;
   t.khi = min(t.p0 + t.ntok, a.maxlen);
   t.klo = max(t.p0 - a.window + 1, (int64_t)0);
   t.c0 = t.klo & ~(int64_t)31;
-  t.nsp = t.khi > t.klo ? (int)sdc_cdiv(t.khi - t.c0, sp.C) : 0;
+  // as many parts as there is room for, from the keys there are
+  const int nk = t.khi > t.klo ? (int)(t.khi - t.c0) : 0;
+  t.C = max(sp.C, ((nk + sp.S - 1) / sp.S + 127) & ~127);
+  t.nsp = (nk + t.C - 1) / t.C;
+}
+__device__ __forceinline__ bool find_tile(const AttendArgs& a, const Split& sp, int id, Tile& t) {
+  t.hb = id % sp.NHB;
+  id /= sp.NHB;
+  t.hk = id % a.Hkv;
+  id /= a.Hkv;
+  Request rq;
+  if (sp.slots) {
+    t.r = id / sp.slots;
+    if (t.r >= a.st.R) return false;
+    rq = sdc_request(a.st, t.r);
+    if (rq.q1 - rq.q0 > (int64_t)sp.slots * sp.TB) return false;
+    t.tok0 = rq.q0 + (int64_t)(id - t.r * sp.slots) * sp.TB;
+  } else {
+    t.r = sdc_request_of(a.st, id, sp.TB, 1);
+    if (t.r < 0) return false;
+    rq = sdc_request(a.st, t.r);
+    if (t.r < a.st.R && rq.q1 - rq.q0 <= sp.few) return false;
+    t.tok0 = rq.q0 + (id - ((int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r)) * sp.TB;
+  }
+  if (t.tok0 < rq.q0 || t.tok0 >= rq.q1) return false;
+  find_keys(a, sp, rq, t);
   return true;
 }
 
@@ -230,7 +254,7 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
     }
     return;
   }
-  const int64_t a0 = t.c0 + (int64_t)s * sp.C, a1 = min(t.khi, a0 + sp.C);
+  const int64_t a0 = t.c0 + (int64_t)s * t.C, a1 = min(t.khi, a0 + t.C);
   const int64_t fp = (uint32_t)a0 / (uint32_t)N;
   const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
 
@@ -513,76 +537,624 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
   }
 }
 
-// The parts of a tile joined, in their order.
-__global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split sp) {
-  const int tid = threadIdx.x, orow = tid >> 4, D = a.D;
+// ---------------------------------------------------------------------------------------------- many query rows
+// Waves of a workgroup, 32 query rows each: a head of 256 needs all 512 registers of a lane.
+constexpr int tall_waves(int64_t D) { return D > 128 ? 4 : 8; }
+
+// The largest of both lanes (l, l + 32) that share a query row, and their sum.
+__device__ __forceinline__ float over_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+__device__ __forceinline__ float over_halves_sum(float v) { return v + __shfl_xor(v, 32); }
+
+// Tiles of up to 256 query rows over a part of their keys, KT keys at a time.  The workgroup widens a tile of codes to
+// fp16 (exact) once, into LDS, keys row by row and values transposed; each wave then reads them as A fragments of
+// v_mfma_f32_32x32x16_f16.  S^T = K Q^T leaves a lane with one query row (l % 32) and keys 8 j + 4 (l / 32) + i; that is
+// the B operand of O^T = V^T P^T if a value row's 16 keys are stored in the order 0-3, 8-11, 4-7, 12-15, so the
+// probabilities never leave their lane.  The next tile's codes are loaded before a tile's products and widened after them,
+// into the other buffer: one barrier a tile.
+//
+// The softmax is what the matrix cores wait for (a score takes 4 D / 1024 cycles of them, and each VALU instruction a
+// 16th), so its common case is short: keys of a group (16, or 4 where a page holds no multiple of 16) share their scales, and
+// with y = x + log2 vs the product p vs is 2^(y - m): one fused multiply-add and one exponential a score; m follows the
+// largest y, and the sum takes the group's sum over vs.  Tiles that some row sees only in part, and scales that are zero, not
+// finite or out of proportion, take the general form.  Rounding of the probabilities and their units: as kv_attend_rows.
+template <int CT, int DP, int PN>
+__global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_attend_tiles(AttendArgs a, Split sp) {
+  constexpr int KT = DP > 128 ? 32 : 64, KB = KT / 32;                  // keys of a tile, blocks of 32
+  constexpr int NS = DP / 16, ND = DP / 32;                             // depth steps of a score, row blocks of the output
+  constexpr int KP = 2 * DP + 16, VP = 2 * KT + 16;                     // row pitches in bytes
+  constexpr int NW = tall_waves(DP), TALL = 32 * NW, HT = 32 * NW;      // half of the threads load keys, half values
+  // reads of a key and of a thread, 16 codes each; columns of 4 codes of a value, units (8 keys x 4 codes) of a thread
+  // (sized so that what a wave reads lies in one page where a page holds multiples of 16 keys)
+  constexpr int KC = DP == 96 ? 8 : DP / 16, KU = (KT * KC + HT - 1) / HT;
+  constexpr int VC = DP <= 96 ? 32 : DP / 4, VUN = KT / 8 * VC, VU = (VUN + HT - 1) / HT;
+  constexpr int NX = 4 * KU > 8 * VU ? 4 * KU : 8 * VU;
+  constexpr float BIAS = 13.f;
+  struct Stage {
+    uint8_t k[KT * KP];
+    uint8_t v[DP * VP];
+    float4 sc[KT];                             // of each key, as of its page
+  };
+  __shared__ Stage st[2];
+  __shared__ int32_t pg[MAXP];
+  __shared__ float4 ps[MAXP];                  // of each page: |ks|, log2 vs, 1 / vs, the factor on the stored values
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int D = a.D, N = a.st.N;
+  const int s = blockIdx.x % sp.S, tile = (int)(sp.tiles - 1 - blockIdx.x / sp.S);  // late tokens, with the most keys, first
   Tile t;
-  if (!find_tile(a, sp, blockIdx.x, t) || t.nsp < 2) return;
-  const int otok = orow / sp.GB, oh = t.hb * sp.GB + orow % sp.GB;
-  if (orow >= sp.GB * sp.TB || otok >= t.ntok || oh >= a.G) return;
-  const int64_t token = t.tok0 + otok, size = (int64_t)ROWS * (D + 2);
-  const int head = t.hk * a.G + oh;
-  const float* rec = sp.part + (int64_t)blockIdx.x * sp.S * size;
-  float m = M0, l = 0.f;
-  for (int s = 0; s < t.nsp; ++s) m = fmaxf(m, rec[s * size + 2 * orow]);
-  for (int s = 0; s < t.nsp; ++s) l += exp2f(rec[s * size + 2 * orow] - m) * rec[s * size + 2 * orow + 1];
-  const int64_t p = t.p0 + otok;
-  const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-  for (int d = tid & 15; d < D; d += 16) {
-    float x = 0.f;
-    for (int s = 0; s < t.nsp; ++s) x += exp2f(rec[s * size + 2 * orow] - m) * rec[s * size + 2 * ROWS + orow * D + d];
-    write_out(a, token, head, d, &x, 1, any ? 1.f / l : 0.f);
+  if (!find_tile(a, sp, tile, t)) return;
+  if (s >= max(t.nsp, 1)) return;
+  // the lane's row (found again at the end, rather than kept)
+  struct Row {
+    int row, tok, head;
+    int64_t token;
+    bool live;
+  };
+  auto row_of = [&]() {
+    int id = threadIdx.x;
+    asm volatile("" : "+v"(id));
+    Row r;
+    r.row = 32 * (id >> 6) + (id & 31);
+    r.tok = r.row / sp.GB;
+    const int hd = t.hb * sp.GB + r.row % sp.GB;
+    r.live = r.row < sp.GB * sp.TB && r.tok < t.ntok && hd < a.G;
+    r.token = t.tok0 + (r.live ? r.tok : 0);
+    r.head = t.hk * a.G + (r.live ? hd : 0);
+    return r;
+  };
+  auto put = [&](const Row& r, int d, float x0, float x1, float x2, float x3) {        // four results at element d
+    uint16_t* op = a.o + r.token * a.sot + r.head * a.soh;
+    const bool wide = a.sod == 1 && ((uintptr_t)a.o % 8 | (uint64_t)(a.sot | a.soh) % 4) == 0;
+    uint32_t v[2];
+    if (a.fp16) {
+      v[0] = sdc_to_half<SDC_FP16>(x0) | (uint32_t)sdc_to_half<SDC_FP16>(x1) << 16;
+      v[1] = sdc_to_half<SDC_FP16>(x2) | (uint32_t)sdc_to_half<SDC_FP16>(x3) << 16;
+    } else {
+      v[0] = sdc_to_half<SDC_BF16>(x0) | (uint32_t)sdc_to_half<SDC_BF16>(x1) << 16;
+      v[1] = sdc_to_half<SDC_BF16>(x2) | (uint32_t)sdc_to_half<SDC_BF16>(x3) << 16;
+    }
+    if (wide) *reinterpret_cast<u32x2*>(op + d) = u32x2{v[0], v[1]};
+    else
+      for (int i = 0; i < 4; ++i) op[(d + i) * a.sod] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+  };
+  if (t.nsp == 0) {                            // no row sees a key
+    const Row r = row_of();
+    if (r.live) {
+      for (int d = 4 * h; d < D; d += 8) put(r, d, 0.f, 0.f, 0.f, 0.f);
+      if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = NEG_INF;
+    }
+    return;
   }
-  if (a.lse && (tid & 15) == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l)) * LN2 : NEG_INF;
+  const int64_t a0 = t.c0 + (int64_t)s * t.C, a1 = min(t.khi, a0 + t.C);
+  const int64_t fp = (uint32_t)a0 / (uint32_t)N;
+  const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
+  // The part's pages and their scales.  A page outside the cache is page 0 with scales of NaN.  Value scales that have no
+  // logarithm (0, infinity, NaN) become factors on the widened values, and so do signs.
+  bool flip = false, mul = false;
+  for (int i = tid; i < np; i += 2 * HT) {
+    const int32_t p = a.st.bt[t.r * a.st.sbt + fp + i];
+    const bool in = p >= 0 && p < a.st.NB;
+    const float* scp = a.scales + (in ? (int64_t)p : 0) * a.sb + t.hk * a.sh;
+    const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf(""), v = fabsf(vs);
+    const bool log = v > 0.f && v < __builtin_inff();
+    ps[i] = {fabsf(ks), log ? log2f(v) : 0.f, log ? fminf(1.f / v, 0x1p126f) : 1.f, log ? (vs < 0.f ? -1.f : 1.f) : vs};
+    pg[i] = (in ? p : 0) | (ks < 0.f ? (int32_t)0x80000000 : 0);        // the sign of ks, which the keys take
+    flip |= ks < 0.f;
+    mul |= !log || vs < 0.f;
+  }
+
+  // the queries: fragments of the lane's row, in fp16 after a power of two
+  f16x8 qf[NS];
+  float rf;
+  int64_t prow;                                // the lane's position
+  {
+    const Row r = row_of();
+    const bool live = r.live;
+    prow = t.p0 + min(r.tok, t.ntok - 1);
+    const uint16_t* qp = a.q + r.token * a.sqt + r.head * a.sqh;
+    const bool vec = a.sqd == 1 && ((uintptr_t)a.q % 16 | (uint64_t)(a.sqt | a.sqh) % 8) == 0;
+    u32x4 raw[NS];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      raw[i] = u32x4{0, 0, 0, 0};
+      const int d = 16 * i + 8 * h;
+      if (live && d < D) {
+        if (vec) raw[i] = *reinterpret_cast<const u32x4*>(qp + d);
+        else
+          for (int e = 0; e < 4; ++e)
+            raw[i][e] = (uint32_t)qp[(d + 2 * e) * a.sqd] | (uint32_t)qp[(d + 2 * e + 1) * a.sqd] << 16;
+      }
+    }
+    int e = 0;
+    auto narrow = [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = fabsf(lo_of<DT>(raw[i][j])), y = fabsf(hi_of<DT>(raw[i][j]));
+          amax = fmaxf(amax, fmaxf(x <= 3.3e38f ? x : 0.f, y <= 3.3e38f ? y : 0.f));
+        }
+      amax = over_halves_max(amax);
+      (void)frexpf(amax, &e);
+      e = max(e, -100);
+      const float f = ldexpf(a.scale < 0.f ? -1.f : 1.f, 13 - e);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qf[i][2 * j] = (_Float16)(lo_of<DT>(raw[i][j]) * f);
+          qf[i][2 * j + 1] = (_Float16)(hi_of<DT>(raw[i][j]) * f);
+        }
+    };
+    if (a.fp16) narrow(std::integral_constant<int, SDC_FP16>{});
+    else narrow(std::integral_constant<int, SDC_BF16>{});
+    rf = ldexpf(fabsf(a.scale), e - 13);       // (scores times key scales that are not negative keep their order)
+  }
+  const bool flips = __syncthreads_or(flip), muls = __syncthreads_or(mul);      // (which is 0 or 1, not the values' or)
+  // keys, counted from a0: those of the tile; those that the lane's row sees; those that a row of the wave, and every row of
+  // the wave sees; those that every row of the tile sees
+  auto clip = [](int64_t x) { return (int)max(min(x, (int64_t)1 << 30), -((int64_t)1 << 30)); };
+  const int nk = (int)(a1 - a0), lo0 = clip(t.klo - a0);
+  const int tok_a = 32 * w / sp.GB, tok_b = min((32 * w + 31) / sp.GB, t.ntok - 1);
+  const int rhi = (int)(min(min(prow + 1, a.maxlen), a1) - a0), rlo = clip(prow - a.window + 1 - a0);
+  const uint32_t span = (uint32_t)max(rhi - rlo, 0);
+  const bool busy = tok_a < t.ntok;            // the wave has rows
+  const int whi = busy ? (int)(min(min(t.p0 + tok_b + 1, a.maxlen), a1) - a0) : 0, wlo = clip(t.p0 + tok_a - a.window + 1 - a0);
+  const int fhi = (int)(min(min(t.p0 + tok_a + 1, a.maxlen), a1) - a0), flo = clip(t.p0 + tok_b - a.window + 1 - a0);
+  const int ahi = (int)(min(min(t.p0 + 1, a.maxlen), a1) - a0), alo = clip(t.p0 + t.ntok - a.window - a0);
+  const uint8_t* base = a.kv + t.hk * a.ch;
+
+  const uint32_t cn = (uint32_t)a.cn;          // (N cn is below 2^31)
+  auto place = [&](int key, int& slot) {       // page entry and slot of a key counted from a0
+    const uint32_t loc = (uint32_t)(base0 + key);
+    const int i = PN == 1 && N == 1 ? (int)loc : (int)__umulhi(loc, sp.div);
+    slot = (int)loc - i * N;
+    return min(i, np - 1);
+  };
+  // The first half of the waves loads and widens the keys, the second the values.  Keys outside the tile's, and codes past
+  // the head's, are read from where there is something to read and taken as zeros.
+  const int half = tid & (HT - 1);
+  const bool vals = w >= NW / 2;
+  bool bad = false;
+  const uint32_t in0 = (uint32_t)(nk - lo0);
+  struct Next {
+    uint32_t x[NX];
+  };
+  // a thread's codes: column and first key (of values: keys key0 + (0..3, 8..11)), where they lie in memory and in LDS
+  const int col = vals ? 4 * (half % VC) : 16 * (half % KC), cg0 = half / VC;
+  const int key0 = vals ? 16 * (cg0 >> 1) + 4 * (cg0 & 1) : half / KC;
+  const uint32_t code = vals ? D + min(col, D - 4) : min(col, D - 16);
+  const uint32_t at = (uint32_t)(vals ? 4 * (cg0 & 1) : key0 % 16) * cn + code;
+  // (a value row's chunks of 16 bytes are moved, by d / 16 % 4, so that writes and reads spread over the banks)
+  const int chunk = vals ? 16 * (cg0 ^ ((col >> 4) & 3)) : 2 * col, lds = vals ? col * VP : key0 * KP;
+  const bool pad = col >= D;
+  auto row_at = [&](int key) {
+    int slot;
+    const int e = place(key, slot);
+    return base + (int64_t)(pg[e] & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
+  };
+  auto group_at = [&](int key) {               // (a wave's keys are in one page, and key, a multiple of 16, the same for all lanes)
+    int slot;
+    const int e = place(__builtin_amdgcn_readfirstlane(key), slot);
+    return base + (int64_t)(__builtin_amdgcn_readfirstlane(pg[e]) & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
+  };
+  auto load = [&](int k0, Next& n) {
+    if (!vals) {
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const int key = k0 + key0 + HT / KC * u;
+        u32x4 x;
+        if constexpr (PN == 16) x = *reinterpret_cast<const u32x4*>(group_at(key & ~15) + (HT / KC * u % 16) * cn + at);
+        else x = *reinterpret_cast<const u32x4*>(row_at(key) + code);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n.x[4 * u + i] = x[i];
+      }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < VU; ++u) {
+      const int key = k0 + key0 + 8 * (HT / VC) * u;
+      if (VUN < HT && half >= VUN) continue;
+      if constexpr (PN == 16) {
+        const uint8_t* p = group_at(key & ~15);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          n.x[8 * u + i] = *reinterpret_cast<const uint32_t*>(p + (i % 4 + 8 * (i / 4)) * cn + at);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          n.x[8 * u + i] = *reinterpret_cast<const uint32_t*>(row_at(key + i % 4 + 8 * (i / 4)) + code);
+      }
+    }
+  };
+  auto store = [&](int k0, Next& n, Stage& d) {
+    const bool whole = k0 >= lo0 && k0 + KT <= nk;
+    if (!vals) {
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const int key = k0 + key0 + HT / KC * u;
+        if (DP == 96 && col >= DP) continue;
+        if ((!whole && (uint32_t)(key - lo0) >= in0) || pad) n.x[4 * u] = n.x[4 * u + 1] = n.x[4 * u + 2] = n.x[4 * u + 3] = 0u;
+        f16x8 p0 = widen8<CT>(n.x[4 * u], n.x[4 * u + 1]), p1 = widen8<CT>(n.x[4 * u + 2], n.x[4 * u + 3]);
+        if (flips) {
+          int slot;
+          const _Float16 f = pg[place(key, slot)] < 0 ? (_Float16)-1.f : (_Float16)1.f;
+          p0 *= f;
+          p1 *= f;
+        }
+        f16x8* p = reinterpret_cast<f16x8*>(d.k + lds + chunk + HT / KC * u * KP);
+        p[0] = p0;
+        p[1] = p1;
+      }
+      return;
+    }
+    const bool part = k0 < alo || k0 + KT > ahi;
+#pragma unroll
+    for (int u = 0; u < VU; ++u) {
+      const int vkey = k0 + key0 + 8 * (HT / VC) * u;
+      if ((VUN < HT && half >= VUN) || (4 * VC > DP && col >= DP)) continue;
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((uint32_t)(vkey + i % 4 + 8 * (i / 4) - lo0) >= in0) n.x[8 * u + i] = 0u;
+      }
+      if (pad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n.x[8 * u + i] = 0u;
+      }
+      // values that are NaN, where some row may not see them (0 times NaN would reach it): left to the end
+      if (CT == SDC_CACHE_E4M3 && part) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t z = nan_codes(n.x[8 * u + i]);
+          n.x[8 * u + i] &= ~((z >> 7) * 0xFFu);
+          bad |= z != 0;
+        }
+      }
+      uint32_t lo[4], hi[4];
+      transpose4(n.x + 8 * u, lo);
+      transpose4(n.x + 8 * u + 4, hi);
+      f16x8 f = {};
+      if (muls) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = vkey + i % 4 + 8 * (i / 4);
+          int slot;
+          const int e = place(key, slot);
+          float x = (uint32_t)(key - lo0) < in0 ? ps[e].w : 1.f;
+          if (part && !(fabsf(x) <= 1.f)) {
+            x = 0.f;
+            bad = true;
+          }
+          f[i] = (_Float16)x;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f16x8 v = widen8<CT>(lo[e], hi[e]);
+        if (muls) v *= f;
+        *reinterpret_cast<f16x8*>(d.v + lds + e * VP + (chunk ^ (16 * (HT / VC) * u))) = v;
+      }
+    }
+    if (half < KT) {
+      int slot;
+      const int e = place(k0 + half, slot);
+      d.sc[half] = ps[e];
+    }
+  };
+
+  f32x16 o[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  float m = M0, l = 0.f;
+
+  auto follow = [&](float top) {               // the maximum follows the scores when they pass it by 2 (fp16 has room for that)
+    if (__any(top > m + 2.f)) {
+      const float mn = fmaxf(m, over_halves_max(top));
+      const float f = exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n] *= f;
+      m = mn;
+    }
+  };
+  // where a lane's fragments lie: row c of a block; chunk (2 j + h) ^ (d / 16 % 4) of element d = 32 n + c
+  const int klane = c * KP + 16 * h, vlane = c * VP + 16 * (h ^ (c >> 4));
+  auto compute = [&](int k0, const Stage& d) {
+    f32x16 x[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(d.k + klane + 32 * b * KP + 32 * i);
+        x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], x[b], 0, 0, 0);
+      }
+    }
+    f16x8 pf[KT / 16];
+    const bool edge = k0 < flo || k0 + KT > fhi;
+    uint32_t seen = 0;
+    auto softmax = [&](auto masked) {
+      constexpr bool EDGE = decltype(masked)::value;
+      constexpr int GE = PN == 16 ? 8 : PN, NG = 16 * KB / GE;          // a lane's scores of a group, groups
+      const float4* scp = d.sc + (PN == 16 ? 0 : 4 * h);
+      auto scales = [&](int j0) { return scp[PN == 16 ? 2 * j0 : 32 * (j0 / 16) + 8 * (j0 % 16 / 4) + j0 % 4]; };
+      float top = NEG_INF;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int j0 = g * GE;
+        const float4 sc = scales(j0);
+        float z = x[j0 / 16][j0 % 16];
+#pragma unroll
+        for (int i = 1; i < GE; ++i) z = fmaxf(z, x[(j0 + i) / 16][(j0 + i) % 16]);
+        top = fmaxf(top, fmaf(z, sc.x * rf, fmaxf(sc.y, -90.f)));
+      }
+      follow(top);
+      if constexpr (PN < 16) asm volatile("" ::: "memory");             // (read again rather than kept)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float4 sc = scales(g * GE);
+        const float cs = sc.x * rf, b0 = sc.y - m + BIAS;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < GE; ++i) {
+          const int j = g * GE + i;
+          float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs, b0));
+          if constexpr (EDGE) p = seen >> j & 1 ? p : 0.f;
+          sum += p;
+          pf[j / 8][j % 8] = (_Float16)p;
+        }
+        l = fmaf(sum, sc.z, l);
+      }
+    };
+    if (!edge) softmax(std::false_type{});
+    else {
+      const uint32_t from = (uint32_t)(k0 + 4 * h - rlo);
+#pragma unroll
+      for (int j = 0; j < 16 * KB; ++j) {
+        const bool in = from + (uint32_t)(32 * (j / 16) + 8 * (j % 16 / 4) + j % 4) < span;
+        seen |= in ? 1u << j : 0u;
+        x[j / 16][j % 16] = in ? x[j / 16][j % 16] : NEG_INF;
+      }
+      softmax(std::true_type{});
+    }
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+#pragma unroll
+      for (int j = 0; j < KT / 16; ++j) {
+        const f16x8 vf = *reinterpret_cast<const f16x8*>(d.v + vlane + 32 * n * VP + 32 * (j ^ (n & 1)));
+        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[j], o[n], 0, 0, 0);
+      }
+    }
+  };
+
+  Next n;
+  load(0, n);
+  store(0, n, st[0]);
+  __syncthreads();
+  for (int k = 0, b = 0; k < nk; k += KT, b ^= 1) {
+    const bool more = k + KT < nk;
+    if (more) load(k + KT, n);
+    if (k < whi && k + KT > wlo) compute(k, st[b]);
+    if (more) store(k + KT, n, st[b ^ 1]);
+    __syncthreads();
+  }
+
+  if (__syncthreads_or(bad)) {                 // values that were left out: NaN for the rows that see them
+    for (int key = max(lo0, rlo); key < rhi; ++key) {
+      const int k0 = key / KT * KT;
+      if (!(k0 < alo || k0 + KT > ahi)) continue;
+      int slot;
+      const int e = place(key, slot);
+      const uint8_t* vp = base + (int64_t)(pg[e] & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn + D;
+      const bool all = !(fabsf(ps[e].w) <= 1.f);
+#pragma unroll
+      for (int q = 0; q < ND; ++q)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int d = 32 * q + 8 * (i / 4) + 4 * h;
+          const uint32_t z = all ? ~0u : CT == SDC_CACHE_E4M3 && d < D ? nan_codes(*reinterpret_cast<const uint32_t*>(vp + d)) : 0u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[q][i + j] = z >> (8 * j + 7) & 1 ? __builtin_nanf("") : o[q][i + j];
+        }
+    }
+  }
+  l = over_halves_sum(l);
+  const Row r = row_of();
+  if (!r.live) return;
+  if (t.nsp == 1) {
+    // (a row with keys whose scores are all -inf: 0 / 0)
+    const int64_t p = t.p0 + r.tok;
+    const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
+    const float f = 1.f / l;
+#pragma unroll
+    for (int q = 0; q < ND; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * q + 8 * i + 4 * h;
+        if (d < D) put(r, d, any ? o[q][4 * i] * f : 0.f, any ? o[q][4 * i + 1] * f : 0.f, any ? o[q][4 * i + 2] * f : 0.f,
+                       any ? o[q][4 * i + 3] * f : 0.f);
+      }
+    if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = any ? (m + log2f(l) - BIAS) * LN2 : NEG_INF;
+  } else {
+    float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + 2);
+    if (h == 0) {
+      rec[2 * r.row] = m;
+      rec[2 * r.row + 1] = l * 0x1p-13f;
+    }
+#pragma unroll
+    for (int q = 0; q < ND; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * q + 8 * i + 4 * h;
+        if (d < D)
+          *reinterpret_cast<f32x4*>(rec + 2 * TALL + r.row * D + d) =
+              f32x4{o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]} * 0x1p-13f;
+      }
+  }
+}
+
+// The parts joined, in their order: a wave for each (token, head), whose parts' weights lie over the lanes.  `all`: every
+// token of the call; else those of the requests that kv_attend_rows takes beside chunks.
+__global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split rows, Split tiles, int all) {
+  const int lane = threadIdx.x & 63, D = a.D;
+  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = id / a.Hq;
+  const int head = (int)(id - k * a.Hq), hd = head % a.G;
+  Tile t;
+  Request rq;
+  int64_t token = k;
+  if (all) {
+    if (token >= a.st.T) return;
+    t.r = sdc_request_of(a.st, token, 1, 0);
+    if (t.r < 0 || t.r >= a.st.R) return;
+    rq = sdc_request(a.st, t.r);
+    if (token >= rq.q1) return;
+  } else {
+    t.r = (int)(k / tiles.few);
+    if (t.r >= a.st.R) return;
+    rq = sdc_request(a.st, t.r);
+    token = rq.q0 + (k - (int64_t)t.r * tiles.few);
+    if (rq.q1 - rq.q0 > tiles.few || token >= rq.q1) return;
+  }
+  const Split& sp = tiles.few && rq.q1 - rq.q0 > tiles.few ? tiles : rows;
+  const int tt = (int)(token - rq.q0) / sp.TB, tok = (int)(token - rq.q0) - tt * sp.TB;
+  t.hk = head / a.G;
+  t.hb = hd / sp.GB;
+  t.tok0 = rq.q0 + (int64_t)tt * sp.TB;
+  find_keys(a, sp, rq, t);
+  if (t.nsp < 2) return;
+  const int row = tok * sp.GB + hd - t.hb * sp.GB;
+  const int64_t first = sp.slots ? (int64_t)t.r * sp.slots : (int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r;
+  const int64_t tile = ((first + tt) * a.Hkv + t.hk) * sp.NHB + t.hb, size = (int64_t)sp.rows * (D + 2);
+  const float* rec = sp.part + tile * sp.S * size;
+  float m = M0;
+  for (int s = lane; s < t.nsp; s += 64) m = fmaxf(m, rec[s * size + 2 * row]);
+  m = wave_max_f32_dpp(m);
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  const bool on = 4 * lane < D;
+  for (int b = 0; b < t.nsp; b += 64) {
+    const int n = min(64, t.nsp - b);
+    float f = 0.f;
+    if (lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(rec + (b + lane) * size + 2 * row);
+      f = exp2f(ml.x - m);
+      l += f * ml.y;
+    }
+    const float* p = rec + b * size + 2 * sp.rows + row * D + 4 * (on ? lane : 0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
+      const f32x4 v = *reinterpret_cast<const f32x4*>(p + s * size);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = fmaf(fs, v[i], x[i]);
+    }
+  }
+  l = wave_sum_f32_dpp(l);
+  const int64_t p = t.p0 + tok;
+  const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
+  if (on) write_out(a, token, head, 4 * lane, x, 4, any ? 1.f / l : 0.f);
+  if (a.lse && lane == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l)) * LN2 : NEG_INF;
 }
 
 // The tiles and parts of a call, from its sizes alone.
-Split plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t N, int64_t most) {
+struct Plan {
+  Split rows, tiles;
+  bool tall;                                   // kv_attend_tiles takes the requests of more than tiles.few tokens
+};
+constexpr int FEW = 2;                         // kv_attend_rows takes requests of up to so many of its tiles, beside chunks
+Split split_of(int rows, int64_t G, int64_t N) {
   Split sp{};
-  sp.GB = (int)std::min<int64_t>(G, ROWS);
-  sp.NHB = (int)sdc_cdiv(G, ROWS);
-  sp.TB = std::max(1, ROWS / sp.GB);
-  sp.tiles = (T / sp.TB + R + 1) * Hkv * sp.NHB;
-  const int64_t busy = std::max<int64_t>(1, std::min(T, T / sp.TB + R) * Hkv * sp.NHB);
-  // parts of at least 256 keys, as many as fill the chip about three times
-  const int64_t want = std::max<int64_t>(1, 1024 / busy);
-  int64_t C = std::max<int64_t>(256, sdc_cdiv(sdc_cdiv(most + 31, want), 128) * 128);
-  C = std::min(C, std::max<int64_t>(128, (MAXP - 2) * N / 128 * 128));
-  C = std::min<int64_t>(C, 16384);
-  sp.C = (int)C;
-  sp.S = (int)std::max<int64_t>(1, sdc_cdiv(most + 31, C));
+  sp.rows = rows;
+  sp.GB = (int)std::min<int64_t>(G, rows);
+  sp.NHB = (int)sdc_cdiv(G, rows);
+  sp.TB = std::max(1, rows / sp.GB);
   sp.div = N == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + N - 1) / N);
   return sp;
 }
-int64_t part_bytes(const Split& sp, int64_t D) {
-  return sp.S == 1 ? 0 : sp.tiles * sp.S * ROWS * (D + 2) * 4;
+// Parts of at least `least` keys, as many as bring `busy` tiles to `want` workgroups; no part has more pages than a
+// workgroup's table.
+void cut(Split& sp, int64_t busy, int64_t want, int64_t least, int64_t keys, int64_t N) {
+  const int64_t most = std::min<int64_t>(16384, std::max<int64_t>(128, (MAXP - 2) * N / 128 * 128));
+  sp.C = (int)std::min(least, most);
+  keys += 31;
+  const int64_t s = std::min(std::max<int64_t>(1, want / std::max<int64_t>(1, busy)), sdc_cdiv(keys, sp.C));
+  // (a tile's keys over S parts, rounded up to 128, must stay within `most`)
+  sp.S = (int)std::max<int64_t>({1, s, sdc_cdiv(keys, most)});
 }
-// keys a tile's rows can see together
-int64_t most_keys(int64_t max_len, int64_t window) { return window > 0 ? std::min(max_len, window + ROWS) : max_len; }
+Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, int64_t max_len, int64_t window) {
+  Plan p{};
+  // keys a tile's rows can see together
+  auto keys = [&](const Split& sp) { return window > 0 ? std::min(max_len, window + sp.TB) : max_len; };
+  p.rows = split_of(ROWS, G, N);
+  p.tiles = split_of(32 * tall_waves(D), G, N);
+  // more tokens than requests: some have a chunk
+  p.tall = T > R && T > FEW * p.rows.TB;
+  if (p.tall) {
+    p.tiles.few = p.rows.TB * FEW;
+    p.rows.slots = FEW;
+    p.tiles.tiles = (T / p.tiles.TB + R + 1) * Hkv * p.tiles.NHB;
+    cut(p.tiles, (T / p.tiles.TB + 1) * Hkv * p.tiles.NHB, 512, 512, keys(p.tiles), N);
+    p.rows.tiles = R * FEW * Hkv * p.rows.NHB;
+    cut(p.rows, R * Hkv * p.rows.NHB, 1024, 256, keys(p.rows), N);
+  } else {
+    p.rows.tiles = (T / p.rows.TB + R + 1) * Hkv * p.rows.NHB;
+    cut(p.rows, std::min(T, T / p.rows.TB + R) * Hkv * p.rows.NHB, 1024, 256, keys(p.rows), N);
+  }
+  return p;
+}
+int64_t part_bytes(const Split& sp, int64_t D) { return sp.S <= 1 ? 0 : sp.tiles * sp.S * sp.rows * (D + 2) * 4; }
 
+int launch_join(const AttendArgs& a, const Plan& p, hipStream_t stream) {
+  if (p.rows.S == 1 && p.tiles.S <= 1) return SDC_OK;
+  const bool all = !p.tall || p.tiles.S > 1;
+  const int64_t blocks = sdc_cdiv((all ? a.st.T : (int64_t)a.st.R * p.tiles.few) * a.Hq, 4);
+  if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
+  if (blocks == 0) return SDC_OK;
+  SdcProf prof("kv_attend_join", stream);
+  hipLaunchKernelGGL(kv_attend_join, dim3((unsigned)blocks), dim3(256), 0, stream, a, p.rows, p.tiles, (int)all);
+  SDC_LAUNCH_CHECK();
+  return SDC_OK;
+}
 template <int CT, int DP>
 int launch_rows(const AttendArgs& a, const Split& sp, hipStream_t stream) {
   const int64_t blocks = sp.tiles * sp.S;
   if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
-  {
-    SdcProf prof("kv_attend", stream);
-    if (a.st.N % 16 == 0)
-      hipLaunchKernelGGL((kv_attend_rows<CT, DP, 16>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sp);
-    else
-      hipLaunchKernelGGL((kv_attend_rows<CT, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sp);
-    SDC_LAUNCH_CHECK();
-  }
-  if (sp.S > 1) {
-    SdcProf prof("kv_attend_join", stream);
-    hipLaunchKernelGGL(kv_attend_join, dim3((unsigned)sp.tiles), dim3(256), 0, stream, a, sp);
-    SDC_LAUNCH_CHECK();
-  }
+  if (blocks == 0) return SDC_OK;
+  SdcProf prof("kv_attend", stream);
+  if (a.st.N % 16 == 0)
+    hipLaunchKernelGGL((kv_attend_rows<CT, DP, 16>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sp);
+  else
+    hipLaunchKernelGGL((kv_attend_rows<CT, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sp);
+  SDC_LAUNCH_CHECK();
   return SDC_OK;
 }
 template <int CT>
 int run_rows(const AttendArgs& a, const Split& sp, hipStream_t stream) {
   if (a.D <= 64) return launch_rows<CT, 64>(a, sp, stream);
   return a.D <= 128 ? launch_rows<CT, 128>(a, sp, stream) : launch_rows<CT, 256>(a, sp, stream);
+}
+template <int CT, int DP>
+int launch_tiles(const AttendArgs& a, const Split& sp, hipStream_t stream) {
+  const int64_t blocks = sp.tiles * sp.S;
+  if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
+  SdcProf prof("kv_attend_tiles", stream);
+  const dim3 grid((unsigned)blocks), threads(64 * tall_waves(DP));
+  if (a.st.N % 16 == 0) hipLaunchKernelGGL((kv_attend_tiles<CT, DP, 16>), grid, threads, 0, stream, a, sp);
+  else if (a.st.N % 4 == 0) hipLaunchKernelGGL((kv_attend_tiles<CT, DP, 4>), grid, threads, 0, stream, a, sp);
+  else hipLaunchKernelGGL((kv_attend_tiles<CT, DP, 1>), grid, threads, 0, stream, a, sp);
+  SDC_LAUNCH_CHECK();
+  return SDC_OK;
+}
+template <int CT>
+int run_tiles(const AttendArgs& a, const Split& sp, hipStream_t stream) {
+  if (a.D <= 64) return launch_tiles<CT, 64>(a, sp, stream);
+  if (a.D <= 96) return launch_tiles<CT, 96>(a, sp, stream);
+  return a.D <= 128 ? launch_tiles<CT, 128>(a, sp, stream) : launch_tiles<CT, 256>(a, sp, stream);
 }
 
 template <int DT>
@@ -603,7 +1175,8 @@ int run(int cache, const AttendArgs& a, hipStream_t stream) {
 extern "C" int64_t sdc_kv_attend_workspace(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t N,
                                            int64_t max_len, int64_t window) {
   if (T < 1 || R < 0 || Hkv < 1 || Hq < Hkv || D < 1 || N < 1 || max_len < 0 || T > 0x3FFFFFFF || R > 0x0FFFFFFF) return 0;
-  return part_bytes(plan(T, R, Hkv, Hq / Hkv, N, most_keys(max_len, window)), D);
+  const Plan p = plan(T, R, Hkv, Hq / Hkv, D, N, max_len, window);
+  return part_bytes(p.rows, D) + part_bytes(p.tiles, D);
 }
 
 extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, int64_t sqh, int64_t sqd, void* o,
@@ -632,11 +1205,18 @@ extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, i
   a.window = window > 0 ? window : (int64_t)1 << 40;
   a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.D = (int)D; a.fp16 = dtype == SDC_FP16;
   // the tiled kernels read 16 codes at a time, and divide by N by a product (exact up to this many slots)
-  if (D % 16 == 0 && N <= 4096 && ((uintptr_t)kv | (uintptr_t)(cb | ch | cn)) % 16 == 0) {
-    Split sp = plan(T, R, Hkv, a.G, N, most_keys(max_len, window));
-    sp.part = (float*)workspace;
-    if (workspace_bytes < part_bytes(sp, D) || (sp.S > 1 && !workspace)) return SDC_EWORKSPACE;
-    return cache == SDC_CACHE_E4M3 ? run_rows<SDC_CACHE_E4M3>(a, sp, stream) : run_rows<SDC_CACHE_I8>(a, sp, stream);
+  if (D % 16 == 0 && N <= 4096 && cn >= 0 && cn < (1 << 19) && ((uintptr_t)kv | (uintptr_t)(cb | ch | cn)) % 16 == 0) {
+    Plan p = plan(T, R, Hkv, a.G, D, N, max_len, window);
+    const int64_t first = part_bytes(p.rows, D), need = first + part_bytes(p.tiles, D);
+    if (workspace_bytes < need || (need && !workspace)) return SDC_EWORKSPACE;
+    p.rows.part = (float*)workspace;
+    p.tiles.part = (float*)((uint8_t*)workspace + first);
+    int rc = SDC_OK;
+    if (p.tall)
+      rc = cache == SDC_CACHE_E4M3 ? run_tiles<SDC_CACHE_E4M3>(a, p.tiles, stream) : run_tiles<SDC_CACHE_I8>(a, p.tiles, stream);
+    if (rc == SDC_OK)
+      rc = cache == SDC_CACHE_E4M3 ? run_rows<SDC_CACHE_E4M3>(a, p.rows, stream) : run_rows<SDC_CACHE_I8>(a, p.rows, stream);
+    return rc == SDC_OK ? launch_join(a, p, stream) : rc;
   }
   return dtype == SDC_BF16 ? run<SDC_BF16>(cache, a, stream) : run<SDC_FP16>(cache, a, stream);
 }
