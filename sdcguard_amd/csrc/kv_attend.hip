@@ -542,8 +542,14 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
 constexpr int tall_waves(int64_t D) { return D > 128 ? 4 : 8; }
 
 // The largest of both lanes (l, l + 32) that share a query row, and their sum.
-__device__ __forceinline__ float over_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
-__device__ __forceinline__ float over_halves_sum(float v) { return v + __shfl_xor(v, 32); }
+__device__ __forceinline__ float over_halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float over_halves_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // Tiles of up to 256 query rows over a part of their keys, KT keys at a time.  The workgroup widens a tile of codes to
 // fp16 (exact) once, into LDS, keys row by row and values transposed; each wave then reads them as A fragments of
@@ -629,18 +635,20 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   const int64_t fp = (uint32_t)a0 / (uint32_t)N;
   const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
   // The part's pages and their scales.  A page outside the cache is page 0 with scales of NaN.  Value scales that have no
-  // logarithm (0, infinity, NaN) become factors on the widened values, and so do signs.
+  // logarithm (0, infinity, NaN) become factors on the widened values, and so do signs; a key scale of NaN makes the page's
+  // share of the sum and its values NaN.
   bool flip = false, mul = false;
   for (int i = tid; i < np; i += 2 * HT) {
     const int32_t p = a.st.bt[t.r * a.st.sbt + fp + i];
     const bool in = p >= 0 && p < a.st.NB;
     const float* scp = a.scales + (in ? (int64_t)p : 0) * a.sb + t.hk * a.sh;
     const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf(""), v = fabsf(vs);
-    const bool log = v > 0.f && v < __builtin_inff();
-    ps[i] = {fabsf(ks), log ? log2f(v) : 0.f, log ? fminf(1.f / v, 0x1p126f) : 1.f, log ? (vs < 0.f ? -1.f : 1.f) : vs};
+    const bool log = v > 0.f && v < __builtin_inff(), key = ks == ks;
+    ps[i] = {key ? fabsf(ks) : 0.f, log ? log2f(v) : 0.f, !key ? ks : log ? fminf(1.f / v, 0x1p126f) : 1.f,
+             !key ? ks : !log ? vs : vs < 0.f ? -1.f : 1.f};
     pg[i] = (in ? p : 0) | (ks < 0.f ? (int32_t)0x80000000 : 0);        // the sign of ks, which the keys take
     flip |= ks < 0.f;
-    mul |= !log || vs < 0.f;
+    mul |= !log || vs < 0.f || !key;
   }
 
   // the queries: fragments of the lane's row, in fp16 after a power of two
@@ -769,16 +777,20 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       }
     }
   };
-  auto store = [&](int k0, Next& n, Stage& d) {
+  auto store = [&](int k0, Next n, Stage& d) {
     const bool whole = k0 >= lo0 && k0 + KT <= nk;
     if (!vals) {
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         const int key = k0 + key0 + HT / KC * u;
         if (DP == 96 && col >= DP) continue;
-        if ((!whole && (uint32_t)(key - lo0) >= in0) || pad) n.x[4 * u] = n.x[4 * u + 1] = n.x[4 * u + 2] = n.x[4 * u + 3] = 0u;
+        if (!whole || D < DP) {
+          asm volatile("");                    // (a branch: it is the same for all lanes and hardly ever taken)
+          if ((uint32_t)(key - lo0) >= in0 || pad) n.x[4 * u] = n.x[4 * u + 1] = n.x[4 * u + 2] = n.x[4 * u + 3] = 0u;
+        }
         f16x8 p0 = widen8<CT>(n.x[4 * u], n.x[4 * u + 1]), p1 = widen8<CT>(n.x[4 * u + 2], n.x[4 * u + 3]);
         if (flips) {
+          asm volatile("");
           int slot;
           const _Float16 f = pg[place(key, slot)] < 0 ? (_Float16)-1.f : (_Float16)1.f;
           p0 *= f;
@@ -795,14 +807,11 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     for (int u = 0; u < VU; ++u) {
       const int vkey = k0 + key0 + 8 * (HT / VC) * u;
       if ((VUN < HT && half >= VUN) || (4 * VC > DP && col >= DP)) continue;
-      if (!whole) {
+      if (!whole || D < DP) {
+        asm volatile("");
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if ((uint32_t)(vkey + i % 4 + 8 * (i / 4) - lo0) >= in0) n.x[8 * u + i] = 0u;
-      }
-      if (pad) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n.x[8 * u + i] = 0u;
+          if ((uint32_t)(vkey + i % 4 + 8 * (i / 4) - lo0) >= in0 || pad) n.x[8 * u + i] = 0u;
       }
       // values that are NaN, where some row may not see them (0 times NaN would reach it): left to the end
       if (CT == SDC_CACHE_E4M3 && part) {
@@ -816,8 +825,11 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       uint32_t lo[4], hi[4];
       transpose4(n.x + 8 * u, lo);
       transpose4(n.x + 8 * u + 4, hi);
-      f16x8 f = {};
+      f16x8 v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = widen8<CT>(lo[e], hi[e]);
       if (muls) {
+        asm volatile("");
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int key = vkey + i % 4 + 8 * (i / 4);
@@ -828,15 +840,13 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
             x = 0.f;
             bad = true;
           }
-          f[i] = (_Float16)x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j][i] *= (_Float16)x;
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f16x8 v = widen8<CT>(lo[e], hi[e]);
-        if (muls) v *= f;
-        *reinterpret_cast<f16x8*>(d.v + lds + e * VP + (chunk ^ (16 * (HT / VC) * u))) = v;
-      }
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f16x8*>(d.v + lds + e * VP + (chunk ^ (16 * (HT / VC) * u))) = v[e];
     }
     if (half < KT) {
       int slot;
@@ -852,16 +862,6 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
   float m = M0, l = 0.f;
 
-  auto follow = [&](float top) {               // the maximum follows the scores when they pass it by 2 (fp16 has room for that)
-    if (__any(top > m + 2.f)) {
-      const float mn = fmaxf(m, over_halves_max(top));
-      const float f = exp2f(m - mn);
-      l *= f;
-#pragma unroll
-      for (int n = 0; n < ND; ++n) o[n] *= f;
-      m = mn;
-    }
-  };
   // where a lane's fragments lie: row c of a block; chunk (2 j + h) ^ (d / 16 % 4) of element d = 32 n + c
   const int klane = c * KP + 16 * h, vlane = c * VP + 16 * (h ^ (c >> 4));
   auto compute = [&](int k0, const Stage& d) {
@@ -876,52 +876,52 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
         x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], x[b], 0, 0, 0);
       }
     }
-    f16x8 pf[KT / 16];
-    const bool edge = k0 < flo || k0 + KT > fhi;
-    uint32_t seen = 0;
-    auto softmax = [&](auto masked) {
-      constexpr bool EDGE = decltype(masked)::value;
-      constexpr int GE = PN == 16 ? 8 : PN, NG = 16 * KB / GE;          // a lane's scores of a group, groups
-      const float4* scp = d.sc + (PN == 16 ? 0 : 4 * h);
-      auto scales = [&](int j0) { return scp[PN == 16 ? 2 * j0 : 32 * (j0 / 16) + 8 * (j0 % 16 / 4) + j0 % 4]; };
-      float top = NEG_INF;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int j0 = g * GE;
-        const float4 sc = scales(j0);
-        float z = x[j0 / 16][j0 % 16];
-#pragma unroll
-        for (int i = 1; i < GE; ++i) z = fmaxf(z, x[(j0 + i) / 16][(j0 + i) % 16]);
-        top = fmaxf(top, fmaf(z, sc.x * rf, fmaxf(sc.y, -90.f)));
-      }
-      follow(top);
-      if constexpr (PN < 16) asm volatile("" ::: "memory");             // (read again rather than kept)
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float4 sc = scales(g * GE);
-        const float cs = sc.x * rf, b0 = sc.y - m + BIAS;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < GE; ++i) {
-          const int j = g * GE + i;
-          float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs, b0));
-          if constexpr (EDGE) p = seen >> j & 1 ? p : 0.f;
-          sum += p;
-          pf[j / 8][j % 8] = (_Float16)p;
-        }
-        l = fmaf(sum, sc.z, l);
-      }
-    };
-    if (!edge) softmax(std::false_type{});
-    else {
+    if (k0 < flo || k0 + KT > fhi) {           // some rows see some of the keys
       const uint32_t from = (uint32_t)(k0 + 4 * h - rlo);
 #pragma unroll
       for (int j = 0; j < 16 * KB; ++j) {
         const bool in = from + (uint32_t)(32 * (j / 16) + 8 * (j % 16 / 4) + j % 4) < span;
-        seen |= in ? 1u << j : 0u;
         x[j / 16][j % 16] = in ? x[j / 16][j % 16] : NEG_INF;
       }
-      softmax(std::true_type{});
+    }
+    constexpr int GE = PN == 16 ? 8 : PN, NG = 16 * KB / GE;            // a lane's scores of a group, groups
+    const float4* scp = d.sc + (PN == 16 ? 0 : 4 * h);
+    auto scales = [&](int j0) { return scp[PN == 16 ? 2 * j0 : 32 * (j0 / 16) + 8 * (j0 % 16 / 4) + j0 % 4]; };
+    auto factor = [&](float ks) { return fmaxf(ks * rf, 0x1p-126f); };  // (not 0: -inf stays)
+    float top = NEG_INF;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int j0 = g * GE;
+      const float4 sc = scales(j0);
+      float z = x[j0 / 16][j0 % 16];
+#pragma unroll
+      for (int i = 1; i < GE; ++i) z = fmaxf(z, x[(j0 + i) / 16][(j0 + i) % 16]);
+      top = fmaxf(top, fmaf(z, factor(sc.x), fmaxf(sc.y, -90.f)));
+    }
+    // the maximum follows the scores when they pass it by 2 (fp16 has room for that)
+    if (__any(top > m + 2.f)) {
+      const float mn = fmaxf(m, over_halves_max(top));
+      const float f = __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n] *= f;
+      m = mn;
+    }
+    if constexpr (PN < 16) asm volatile("" ::: "memory");               // (scales are read again rather than kept)
+    f16x8 pf[KT / 16];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float4 sc = scales(g * GE);
+      const float cs = factor(sc.x), b0 = sc.y - m + BIAS;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < GE; ++i) {
+        const int j = g * GE + i;
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs, b0));
+        sum += p;
+        pf[j / 8][j % 8] = (_Float16)p;
+      }
+      l = sum == 0.f ? l : fmaf(sum, sc.z, l);
     }
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
