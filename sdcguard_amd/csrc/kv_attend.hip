@@ -666,7 +666,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       raw[i] = u32x4{0, 0, 0, 0};
-      const int d = 16 * i + 8 * h;
+      const int run = 2 * i + h, d = 16 * (run % NS) + 8 * (run / NS);  // (the order in which the keys' codes are stored)
       if (live && d < D) {
         if (vec) raw[i] = *reinterpret_cast<const u32x4*>(qp + d);
         else
@@ -735,8 +735,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   const int key0 = vals ? 16 * (cg0 >> 1) + 4 * (cg0 & 1) : half / KC;
   const uint32_t code = vals ? D + min(col, D - 4) : min(col, D - 16);
   const uint32_t at = (uint32_t)(vals ? 4 * (cg0 & 1) : key0 % 16) * cn + code;
-  // (a value row's chunks of 16 bytes are moved, by d / 16 % 4, so that writes and reads spread over the banks)
-  const int chunk = vals ? 16 * (cg0 ^ ((col >> 4) & 3)) : 2 * col, lds = vals ? col * VP : key0 * KP;
+  const int lds = vals ? col / 4 * VP + 16 * cg0 : key0 * KP + col;
   const bool pad = col >= D;
   auto row_at = [&](int key) {
     int slot;
@@ -796,9 +795,9 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
           p0 *= f;
           p1 *= f;
         }
-        f16x8* p = reinterpret_cast<f16x8*>(d.k + lds + chunk + HT / KC * u * KP);
-        p[0] = p0;
-        p[1] = p1;
+        uint8_t* p = d.k + lds + HT / KC * u * KP;            // (two runs of 8 codes, half a row apart)
+        *reinterpret_cast<f16x8*>(p) = p0;
+        *reinterpret_cast<f16x8*>(p + DP) = p1;
       }
       return;
     }
@@ -846,7 +845,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f16x8*>(d.v + lds + e * VP + (chunk ^ (16 * (HT / VC) * u))) = v[e];
+        *reinterpret_cast<f16x8*>(d.v + lds + e * (DP / 4) * VP + 16 * (HT / VC) * u) = v[e];
     }
     if (half < KT) {
       int slot;
@@ -862,8 +861,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
   float m = M0, l = 0.f;
 
-  // where a lane's fragments lie: row c of a block; chunk (2 j + h) ^ (d / 16 % 4) of element d = 32 n + c
-  const int klane = c * KP + 16 * h, vlane = c * VP + 16 * (h ^ (c >> 4));
+  const int klane = c * KP + 16 * h, vlane = c * VP + 16 * h;           // row c of a block, the half's run of 8
   auto compute = [&](int k0, const Stage& d) {
     f32x16 x[KB];
 #pragma unroll
@@ -927,7 +925,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     for (int n = 0; n < ND; ++n) {
 #pragma unroll
       for (int j = 0; j < KT / 16; ++j) {
-        const f16x8 vf = *reinterpret_cast<const f16x8*>(d.v + vlane + 32 * n * VP + 32 * (j ^ (n & 1)));
+        const f16x8 vf = *reinterpret_cast<const f16x8*>(d.v + vlane + 32 * n * VP + 32 * j);
         o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[j], o[n], 0, 0, 0);
       }
     }
@@ -945,6 +943,31 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     __syncthreads();
   }
 
+  // o[q][i] of a lane is element 4 (p % (DP / 4)) + p / (DP / 4), p = 32 q + 8 (i / 4) + 4 h + i % 4: the values' rows lie in that
+  // order, which gives a lane four adjacent elements (not of 96, whose quarters are no blocks)
+  auto element = [&](int q, int i) {
+    const int p = 32 * q + 8 * (i / 4) + 4 * h + i % 4;
+    return 4 * (p % (DP / 4)) + p / (DP / 4);
+  };
+  auto each = [&](auto use4, auto use1) {
+    if constexpr (DP != 96) {
+      constexpr int B = DP / 128 > 0 ? DP / 128 : 1, E = DP == 64 ? 8 : 16;    // blocks and registers of a quarter's rows
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = DP == 64 ? o[e / 2][i + 8 * (e % 2)] : o[b + B * e][i];
+          use4(element(b, i), x);
+        }
+    } else {
+#pragma unroll
+      for (int q = 0; q < ND; ++q)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) use1(element(q, i), o[q][i]);
+    }
+  };
   if (__syncthreads_or(bad)) {                 // values that were left out: NaN for the rows that see them
     for (int key = max(lo0, rlo); key < rhi; ++key) {
       const int k0 = key / KT * KT;
@@ -956,11 +979,10 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
 #pragma unroll
       for (int q = 0; q < ND; ++q)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int d = 32 * q + 8 * (i / 4) + 4 * h;
-          const uint32_t z = all ? ~0u : CT == SDC_CACHE_E4M3 && d < D ? nan_codes(*reinterpret_cast<const uint32_t*>(vp + d)) : 0u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[q][i + j] = z >> (8 * j + 7) & 1 ? __builtin_nanf("") : o[q][i + j];
+        for (int i = 0; i < 16; ++i) {
+          uint32_t z = all;
+          if constexpr (CT == SDC_CACHE_E4M3) z |= (uint32_t)((vp[min(element(q, i), D - 1)] & 0x7F) == 0x7F);
+          o[q][i] = z ? __builtin_nanf("") : o[q][i];
         }
     }
   }
@@ -972,14 +994,9 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     const int64_t p = t.p0 + r.tok;
     const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
     const float f = 1.f / l;
-#pragma unroll
-    for (int q = 0; q < ND; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 32 * q + 8 * i + 4 * h;
-        if (d < D) put(r, d, any ? o[q][4 * i] * f : 0.f, any ? o[q][4 * i + 1] * f : 0.f, any ? o[q][4 * i + 2] * f : 0.f,
-                       any ? o[q][4 * i + 3] * f : 0.f);
-      }
+    each([&](int d, f32x4 x) {
+      if (d < D) put(r, d, any ? x[0] * f : 0.f, any ? x[1] * f : 0.f, any ? x[2] * f : 0.f, any ? x[3] * f : 0.f);
+    }, [&](int d, float x) { write_out(a, r.token, r.head, d, &x, 1, any ? f : 0.f); });
     if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = any ? (m + log2f(l) - BIAS) * LN2 : NEG_INF;
   } else {
     float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + 2);
@@ -987,15 +1004,11 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       rec[2 * r.row] = m;
       rec[2 * r.row + 1] = l * 0x1p-13f;
     }
-#pragma unroll
-    for (int q = 0; q < ND; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 32 * q + 8 * i + 4 * h;
-        if (d < D)
-          *reinterpret_cast<f32x4*>(rec + 2 * TALL + r.row * D + d) =
-              f32x4{o[q][4 * i], o[q][4 * i + 1], o[q][4 * i + 2], o[q][4 * i + 3]} * 0x1p-13f;
-      }
+    each([&](int d, f32x4 x) {
+      if (d < D) *reinterpret_cast<f32x4*>(rec + 2 * TALL + r.row * D + d) = x * 0x1p-13f;
+    }, [&](int d, float x) {
+      if (d < D) rec[2 * TALL + r.row * D + d] = x * 0x1p-13f;
+    });
   }
 }
 
