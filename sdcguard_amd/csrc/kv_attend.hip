@@ -862,18 +862,31 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   float m = M0, l = 0.f;
 
   const int klane = c * KP + 16 * h, vlane = c * VP + 16 * h;           // row c of a block, the half's run of 8
-  auto compute = [&](int k0, const Stage& d) {
-    f32x16 x[KB];
+  auto products = [&](const uint8_t* k, f32x16* x) {                    // the scores of a tile's keys
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const f16x8 kf = *reinterpret_cast<const f16x8*>(d.k + klane + 32 * b * KP + 32 * i);
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(k + klane + 32 * b * KP + 32 * i);
         x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], x[b], 0, 0, 0);
       }
     }
+  };
+  // the softmax and the values' products of a tile whose scores are x; between its exponentials, the next tile's scores
+  auto finish = [&](int k0, const Stage& d, f32x16* x, const uint8_t* next, f32x16* y) {
+    // Fragments are read AHEAD products before they are used (left to itself the compiler reads one at a time and waits for
+    // it: 320 us instead of XXX), first the keys', then the values', neighbours into different accumulators.
+    constexpr int MK = KB * NS, MV = ND * KT / 16, AHEAD = 4;
+    f16x8 fr[AHEAD];
+    auto fragment = [&](int q) {
+      return *reinterpret_cast<const f16x8*>(q < MK ? next + klane + 32 * (q % KB) * KP + 32 * (q / KB)
+                                                    : d.v + vlane + 32 * ((q - MK) % ND) * VP + 32 * ((q - MK) / ND));
+    };
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) fr[q] = fragment(q);
+    __builtin_amdgcn_sched_barrier(0x6);
     if (k0 < flo || k0 + KT > fhi) {           // some rows see some of the keys
       const uint32_t from = (uint32_t)(k0 + 4 * h - rlo);
 #pragma unroll
@@ -905,42 +918,64 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       for (int n = 0; n < ND; ++n) o[n] *= f;
       m = mn;
     }
-    if constexpr (PN < 16) asm volatile("" ::: "memory");               // (scales are read again rather than kept)
     f16x8 pf[KT / 16];
+    float cs[NG], b0[NG], inv[NG], sum[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float4 sc = scales(g * GE);
-      const float cs = factor(sc.x), b0 = sc.y - m + BIAS;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < GE; ++i) {
-        const int j = g * GE + i;
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs, b0));
-        sum += p;
-        pf[j / 8][j % 8] = (_Float16)p;
-      }
-      l = sum == 0.f ? l : fmaf(sum, sc.z, l);
+      cs[g] = factor(sc.x);
+      b0[g] = sc.y - m + BIAS;
+      inv[g] = sc.z;
+      sum[g] = 0.f;
     }
 #pragma unroll
-    for (int n = 0; n < ND; ++n) {
+    for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int j = 0; j < KT / 16; ++j) {
-        const f16x8 vf = *reinterpret_cast<const f16x8*>(d.v + vlane + 32 * n * VP + 32 * j);
-        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[j], o[n], 0, 0, 0);
+      for (int i = 0; i < 16; ++i) y[b][i] = 0.f;
+#pragma unroll
+    for (int q = 0; q < MK + MV; ++q) {
+      if (q < MK) y[q % KB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[q % AHEAD], qf[q / KB], y[q % KB], 0, 0, 0);
+      else o[(q - MK) % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[q % AHEAD], pf[(q - MK) / ND], o[(q - MK) % ND], 0, 0, 0);
+      if (q + AHEAD < MK + MV) fr[q % AHEAD] = fragment(q + AHEAD);
+      if (q < MK) {
+#pragma unroll
+        for (int j = q * 16 * KB / MK; j < (q + 1) * 16 * KB / MK; ++j) {
+          const int g = j / GE;
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs[g], b0[g]));
+          sum[g] += p;
+          pf[j / 8][j % 8] = (_Float16)p;
+        }
       }
+      __builtin_amdgcn_sched_barrier(0x6);
     }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) l = sum[g] == 0.f ? l : fmaf(sum[g], inv[g], l);
   };
 
+  // In the step of tile t the waves take the values of t and the keys of t + 1, while the values of t + 1 and the keys of t + 2
+  // are loaded and put where the values of t - 1 and the keys of t were.
   Next n;
   load(0, n);
   store(0, n, st[0]);
+  if (!vals && KT < nk) {
+    load(KT, n);
+    store(KT, n, st[1]);
+  }
   __syncthreads();
-  for (int k = 0, b = 0; k < nk; k += KT, b ^= 1) {
-    const bool more = k + KT < nk;
-    if (more) load(k + KT, n);
-    if (k < whi && k + KT > wlo) compute(k, st[b]);
-    if (more) store(k + KT, n, st[b ^ 1]);
+  f32x16 xa[KB], xb[KB];
+  products(st[0].k, xa);
+  __syncthreads();
+  auto step = [&](int k, Stage& d, Stage& e, f32x16* x, f32x16* y) {
+    const int ahead = k + (vals ? KT : 2 * KT);
+    if (ahead < nk) load(ahead, n);
+    if (k < whi && k + KT > wlo) finish(k, d, x, e.k, y);
+    else if (k + KT < whi && k + 2 * KT > wlo) products(e.k, y);
+    if (ahead < nk) store(ahead, n, vals ? e : d);
     __syncthreads();
+  };
+  for (int k = 0; k < nk; k += 2 * KT) {
+    step(k, st[0], st[1], xa, xb);
+    if (k + KT < nk) step(k + KT, st[1], st[0], xb, xa);
   }
 
   // o[q][i] of a lane is element 4 (p % (DP / 4)) + p / (DP / 4), p = 32 q + 8 (i / 4) + 4 h + i % 4: the values' rows lie in that
