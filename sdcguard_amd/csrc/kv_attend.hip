@@ -742,19 +742,29 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     const int e = place(key, slot);
     return base + (int64_t)(pg[e] & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
   };
-  auto group_at = [&](int key) {               // (a wave's keys are in one page, and key, a multiple of 16, the same for all lanes)
+  // Where a wave's keys are in one page its entry is read a step before it is needed (its 16 keys are the same for all lanes).
+  constexpr int KSTEP = HT / KC, VSTEP = 8 * (HT / VC);                 // keys between a thread's reads
+  int entry[KU > VU ? KU : VU];
+  auto group = [&](int k0, int u) { return __builtin_amdgcn_readfirstlane((k0 + key0 + (vals ? VSTEP : KSTEP) * u) & ~15); };
+  auto find = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < (KU > VU ? KU : VU); ++u) {
+      int slot;
+      if (PN == 16) entry[u] = pg[place(group(k0, u), slot)];
+    }
+  };
+  auto group_at = [&](int k0, int u) {
     int slot;
-    const int e = place(__builtin_amdgcn_readfirstlane(key), slot);
-    return base + (int64_t)(__builtin_amdgcn_readfirstlane(pg[e]) & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
+    (void)place(group(k0, u), slot);
+    return base + (int64_t)(__builtin_amdgcn_readfirstlane(entry[u]) & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
   };
   auto load = [&](int k0, Next& n) {
     if (!vals) {
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
-        const int key = k0 + key0 + HT / KC * u;
         u32x4 x;
-        if constexpr (PN == 16) x = *reinterpret_cast<const u32x4*>(group_at(key & ~15) + (HT / KC * u % 16) * cn + at);
-        else x = *reinterpret_cast<const u32x4*>(row_at(key) + code);
+        if constexpr (PN == 16) x = *reinterpret_cast<const u32x4*>(group_at(k0, u) + (KSTEP * u % 16) * cn + at);
+        else x = *reinterpret_cast<const u32x4*>(row_at(k0 + key0 + KSTEP * u) + code);
 #pragma unroll
         for (int i = 0; i < 4; ++i) n.x[4 * u + i] = x[i];
       }
@@ -762,10 +772,10 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     }
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
-      const int key = k0 + key0 + 8 * (HT / VC) * u;
+      const int key = k0 + key0 + VSTEP * u;
       if (VUN < HT && half >= VUN) continue;
       if constexpr (PN == 16) {
-        const uint8_t* p = group_at(key & ~15);
+        const uint8_t* p = group_at(k0, u);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           n.x[8 * u + i] = *reinterpret_cast<const uint32_t*>(p + (i % 4 + 8 * (i / 4)) * cn + at);
@@ -952,25 +962,35 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     for (int g = 0; g < NG; ++g) l = sum[g] == 0.f ? l : fmaf(sum[g], inv[g], l);
   };
 
-  // In the step of tile t the waves take the values of t and the keys of t + 1, while the values of t + 1 and the keys of t + 2
-  // are loaded and put where the values of t - 1 and the keys of t were.
+  // In the step of tile t the waves take the values of t and the keys of t + 1.  At its start the values of t + 1 and the keys of
+  // t + 2, loaded during the step before, are put where the values of t - 1 and the keys of t were.
   Next n;
+  find(0);
   load(0, n);
   store(0, n, st[0]);
-  if (!vals && KT < nk) {
+  if (KT < nk) {
+    find(KT);
     load(KT, n);
-    store(KT, n, st[1]);
+    if (!vals) {
+      store(KT, n, st[1]);
+      if (2 * KT < nk) {
+        find(2 * KT);
+        load(2 * KT, n);
+      }
+    }
   }
+  const int ahead = vals ? KT : 2 * KT;
+  find(ahead + KT);
   __syncthreads();
   f32x16 xa[KB], xb[KB];
   products(st[0].k, xa);
   __syncthreads();
   auto step = [&](int k, Stage& d, Stage& e, f32x16* x, f32x16* y) {
-    const int ahead = k + (vals ? KT : 2 * KT);
-    if (ahead < nk) load(ahead, n);
+    if (k + ahead < nk) store(k + ahead, n, vals ? e : d);
+    if (k + ahead + KT < nk) load(k + ahead + KT, n);
     if (k < whi && k + KT > wlo) finish(k, d, x, e.k, y);
     else if (k + KT < whi && k + 2 * KT > wlo) products(e.k, y);
-    if (ahead < nk) store(ahead, n, vals ? e : d);
+    find(k + ahead + 2 * KT);
     __syncthreads();
   };
   for (int k = 0; k < nk; k += 2 * KT) {
