@@ -120,11 +120,12 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   typedef typename RopeElem<DT>::T E;
   const PagedStep& st = a.st;
   const int N = st.N, D = a.D, tid = threadIdx.x, lane = tid & 63;
-  const int r = sdc_request_of(st, item, N, 2);
+  Request rq;
+  int64_t first;
+  const int r = sdc_find_request(st, item, N, 2, rq, first);
   if (r < 0 || r >= st.R) return;
-  const Request rq = sdc_request(st, r);
   const int64_t pos0 = max(rq.len - (rq.q1 - rq.q0), (int64_t)0);
-  const int64_t w = pos0 / N + (item - ((int64_t)((uint32_t)st.qsl[r] / (uint32_t)N) + 2 * (int64_t)r));
+  const int64_t w = pos0 / N + (item - first);
   const int64_t lo = max(pos0, w * N), hi = min(rq.len, (w + 1) * N);
   if (lo >= hi || w >= st.W) return;
   const int64_t page = st.bt[r * st.sbt + w];
@@ -244,10 +245,10 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t bloc
     const int nt = (int)min((int64_t)TB, te - t0);
     __syncthreads();
     for (int t = tid >> 6; t < nt; t += 4) {                            // a wave per token: its request, its position
-      const int r = sdc_request_of(a.st, t0 + t, 1, 0);
-      int64_t p = -1;
+      Request rq;
+      int64_t first, p = -1;
+      const int r = sdc_find_request(a.st, t0 + t, 1, 0, rq, first);
       if (r >= 0 && r < a.st.R) {
-        const Request rq = sdc_request(a.st, r);
         p = max(t0 + t - rq.q1 + rq.len, (int64_t)0);
       }
       if ((tid & 63) == 0) own[t] = p;

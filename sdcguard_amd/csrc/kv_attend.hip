@@ -67,10 +67,11 @@ __global__ __launch_bounds__(256) void kv_attend_any(AttendArgs a) {
   for (int d = lane; d < D; d += 64) qs[w][d] = half_to_f32<DT>(a.q[t * a.sqt + h * a.sqh + d * a.sqd]);
   sdc_wave_lds_fence();
   if (!live) return;
-  const int r = sdc_request_of(a.st, t, 1, 0);
+  Request rq;
+  int64_t first;
+  const int r = sdc_find_request(a.st, t, 1, 0, rq, first);
   int64_t lo = 0, hi = 0;
   if (r >= 0 && r < a.st.R) {
-    const Request rq = sdc_request(a.st, r);
     hi = min(t - rq.q1 + rq.len + 1, a.maxlen);
     lo = max(t - rq.q1 + rq.len + 1 - a.window, (int64_t)0);
   }
@@ -194,11 +195,11 @@ __device__ __forceinline__ bool find_tile(const AttendArgs& a, const Split& sp, 
     if (rq.q1 - rq.q0 > (int64_t)sp.slots * sp.TB) return false;
     t.tok0 = rq.q0 + (int64_t)(id - t.r * sp.slots) * sp.TB;
   } else {
-    t.r = sdc_request_of(a.st, id, sp.TB, 1);
+    int64_t first;
+    t.r = sdc_find_request(a.st, id, sp.TB, 1, rq, first);
     if (t.r < 0) return false;
-    rq = sdc_request(a.st, t.r);
     if (t.r < a.st.R && rq.q1 - rq.q0 <= sp.few) return false;
-    t.tok0 = rq.q0 + (id - ((int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r)) * sp.TB;
+    t.tok0 = rq.q0 + (id - first) * sp.TB;
   }
   if (t.tok0 < rq.q0 || t.tok0 >= rq.q1) return false;
   find_keys(a, sp, rq, t);
@@ -221,7 +222,7 @@ __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t tok, int 
 // The key scales multiply the scores, the value scales the probabilities, in fp32.  Probabilities are rounded to fp16's
 // 11 bits, in units that put their largest product with a value scale at 2^13 .. 2^15.
 template <int CT, int DP, int PN>
-__global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendArgs a, Split sp) {
   constexpr int KW = DP / 64;                  // 16-byte reads of a key per lane; dwords of a value per lane
   constexpr int NS = DP / 32, ND = DP / 16;    // depth steps of a score, row blocks of the output
   constexpr int QS = DP + 8, OS = DP + 4;      // row pitches in LDS
@@ -258,27 +259,126 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
   const int64_t fp = (uint32_t)a0 / (uint32_t)N;
   const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
 
-  // the part's pages and their scales; a page outside the cache is page 0 with scales of NaN
-  float vmax = 0.f;
+  // the part's pages; a page outside the cache is page 0, marked by its sign
   for (int i = tid; i < np; i += 256) {
     const int32_t page = a.st.bt[t.r * a.st.sbt + fp + i];
-    const bool in = page >= 0 && page < a.st.NB;
-    const float* scp = a.scales + (in ? (int64_t)page : 0) * a.sb + t.hk * a.sh;
+    sh.h.pg[i] = page >= 0 && page < a.st.NB ? page : (int32_t)0x80000000;
+  }
+  // the queries, a row per 16 threads
+  uint32_t qr[ND / 2];
+  {
+    const uint16_t* qp = a.q + (olive ? otoken * a.sqt + ohead * a.sqh : 0);
+    const bool vec = a.sqd == 1 && ((uintptr_t)a.q % 16 | (uint64_t)(a.sqt | a.sqh) % 8) == 0;
+#pragma unroll
+    for (int i = 0; i < ND / 2; ++i) qr[i] = 0u;
+    if (olive && od < D) {
+      if (vec) {                               // (D is a multiple of 16, and ND 4, 8 or 16)
+        constexpr int C = ND / 2 < 4 ? 2 : 4;
+        typedef uint32_t vt __attribute__((ext_vector_type(C)));
+#pragma unroll
+        for (int i = 0; i < ND / 2; i += C) {
+          const vt x = *reinterpret_cast<const vt*>(qp + od + 2 * i);
+#pragma unroll
+          for (int j = 0; j < C; ++j) qr[i + j] = x[j];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < ND / 2; ++i)
+          qr[i] = (uint32_t)qp[(od + 2 * i) * a.sqd] | (uint32_t)qp[(od + 2 * i + 1) * a.sqd] << 16;
+      }
+    }
+  }
+  __syncthreads();
+  const int nk = (int)(a1 - a0);
+  const uint8_t* base = a.kv + t.hk * a.ch;
+  // page entry and slot of a key counted from a0
+  auto place = [&](int key, int& slot) {
+    const uint32_t loc = (uint32_t)(base0 + key);
+    const int i = N == 1 ? (int)loc : (int)__umulhi(loc, sp.div);
+    slot = (int)loc - i * N;
+    return min(i, np - 1);
+  };
+  struct Buf {
+    u32x4 k[2][KW];
+    uint32_t v[8][KW];
+    int e[8];                                  // the keys' page entries
+  };
+  auto load = [&](int k0, Buf& b) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      int slot, e;
+      const uint8_t* row;
+      if constexpr (PN == 16) {                // the 16 keys lie in one page
+        e = __builtin_amdgcn_readfirstlane(place(k0 + 16 * u, slot));
+        slot = __builtin_amdgcn_readfirstlane(slot);
+        row = base + (int64_t)(__builtin_amdgcn_readfirstlane(sh.h.pg[e]) & 0x7FFFFFFF) * a.cb + (int64_t)slot * a.cn;
+        const uint8_t* kr = row + c * a.cn + g * (DP / 4);
+#pragma unroll
+        for (int j = 0; j < KW; ++j)
+          b.k[u][j] = g * (DP / 4) + 16 * j < D ? *reinterpret_cast<const u32x4*>(kr + 16 * j) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* vr = row + (4 * g + i) * a.cn + D + c * (DP / 16);
+          b.e[4 * u + i] = e;
+          typedef uint32_t vt __attribute__((ext_vector_type(KW)));
+          if constexpr (KW == 1) b.v[4 * u + i][0] = c * (DP / 16) < D ? *reinterpret_cast<const uint32_t*>(vr) : 0u;
+          else {
+            vt x = {};
+            if (c * (DP / 16) < D) x = *reinterpret_cast<const vt*>(vr);
+#pragma unroll
+            for (int j = 0; j < KW; ++j) b.v[4 * u + i][j] = x[j];
+          }
+        }
+      } else {
+        e = place(k0 + 16 * u + c, slot);
+        row = base + (int64_t)(sh.h.pg[e] & 0x7FFFFFFF) * a.cb + (int64_t)slot * a.cn;
+#pragma unroll
+        for (int j = 0; j < KW; ++j)
+          b.k[u][j] = g * (DP / 4) + 16 * j < D ? *reinterpret_cast<const u32x4*>(row + g * (DP / 4) + 16 * j) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e = place(k0 + 16 * u + 4 * g + i, slot);
+          b.e[4 * u + i] = e;
+          const uint8_t* vr = base + (int64_t)(sh.h.pg[e] & 0x7FFFFFFF) * a.cb + (int64_t)slot * a.cn + D + c * (DP / 16);
+#pragma unroll
+          for (int j = 0; j < KW; ++j)
+            b.v[4 * u + i][j] = c * (DP / 16) < D ? *reinterpret_cast<const uint32_t*>(vr + 4 * j) : 0u;
+        }
+      }
+    }
+  };
+
+  Buf b0, b1;
+  int k = 32 * w;
+  if (k < nk) load(k, b0);                     // (on their way while the scales are read and the queries put in place)
+  if (k + 128 < nk) load(k + 128, b1);
+  float vmax = 0.f;
+  for (int i = tid; i < np; i += 256) {
+    const int32_t page = sh.h.pg[i];
+    const float* scp = a.scales + (int64_t)(page & 0x7FFFFFFF) * a.sb + t.hk * a.sh;
     float2 sc = {scp[0], scp[1]};
-    if (!in) sc = {__builtin_nanf(""), __builtin_nanf("")};
-    sh.h.pg[i] = in ? page : 0;
+    if (page < 0) sc = {__builtin_nanf(""), __builtin_nanf("")};
     sh.h.sc[i] = sc;
     const float v = fabsf(sc.y);
     if (v <= 3.0e38f) vmax = fmaxf(vmax, v);
   }
-  // the queries, a row per 16 threads
   {
     float x[ND], amax = 0.f;
-    const uint16_t* qp = a.q + (olive ? otoken * a.sqt + ohead * a.sqh : 0);
+    if (a.fp16) {
+#pragma unroll
+      for (int i = 0; i < ND / 2; ++i) {
+        x[2 * i] = f16_lo(qr[i]);
+        x[2 * i + 1] = f16_hi(qr[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ND / 2; ++i) {
+        x[2 * i] = bf16_lo(qr[i]);
+        x[2 * i + 1] = bf16_hi(qr[i]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-      const uint16_t v = olive && od + i < D ? qp[(od + i) * a.sqd] : (uint16_t)0;
-      x[i] = a.fp16 ? half_to_f32<SDC_FP16>(v) : half_to_f32<SDC_BF16>(v);
       const float f = fabsf(x[i]);
       if (f <= 3.3e38f) amax = fmaxf(amax, f);
     }
@@ -311,72 +411,11 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
   // those that every row of the tile sees
   const int fhi = (int)(min(min(t.p0 + 1, a.maxlen), a1) - a0);
   const int flo = (int)max(min(t.p0 + t.ntok - a.window - a0, (int64_t)1 << 30), -((int64_t)1 << 30));
-  const int nk = (int)(a1 - a0);
 
   f32x4 o[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = M0, l = 0.f;
-  const uint8_t* base = a.kv + t.hk * a.ch;
-
-  // page entry and slot of a key counted from a0
-  auto place = [&](int key, int& slot) {
-    const uint32_t loc = (uint32_t)(base0 + key);
-    const int i = N == 1 ? (int)loc : (int)__umulhi(loc, sp.div);
-    slot = (int)loc - i * N;
-    return min(i, np - 1);
-  };
-  struct Buf {
-    u32x4 k[2][KW];
-    uint32_t v[8][KW];
-    float2 sc[8];
-  };
-  auto load = [&](int k0, Buf& b) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      int slot, e;
-      const uint8_t* row;
-      if constexpr (PN == 16) {                // the 16 keys lie in one page
-        e = __builtin_amdgcn_readfirstlane(place(k0 + 16 * u, slot));
-        slot = __builtin_amdgcn_readfirstlane(slot);
-        const float2 sc = sh.h.sc[e];
-        row = base + (int64_t)__builtin_amdgcn_readfirstlane(sh.h.pg[e]) * a.cb + (int64_t)slot * a.cn;
-        const uint8_t* kr = row + c * a.cn + g * (DP / 4);
-#pragma unroll
-        for (int j = 0; j < KW; ++j)
-          b.k[u][j] = g * (DP / 4) + 16 * j < D ? *reinterpret_cast<const u32x4*>(kr + 16 * j) : u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t* vr = row + (4 * g + i) * a.cn + D + c * (DP / 16);
-          b.sc[4 * u + i] = sc;
-          typedef uint32_t vt __attribute__((ext_vector_type(KW)));
-          if constexpr (KW == 1) b.v[4 * u + i][0] = c * (DP / 16) < D ? *reinterpret_cast<const uint32_t*>(vr) : 0u;
-          else {
-            vt x = {};
-            if (c * (DP / 16) < D) x = *reinterpret_cast<const vt*>(vr);
-#pragma unroll
-            for (int j = 0; j < KW; ++j) b.v[4 * u + i][j] = x[j];
-          }
-        }
-      } else {
-        e = place(k0 + 16 * u + c, slot);
-        row = base + (int64_t)sh.h.pg[e] * a.cb + (int64_t)slot * a.cn;
-#pragma unroll
-        for (int j = 0; j < KW; ++j)
-          b.k[u][j] = g * (DP / 4) + 16 * j < D ? *reinterpret_cast<const u32x4*>(row + g * (DP / 4) + 16 * j) : u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e = place(k0 + 16 * u + 4 * g + i, slot);
-          b.sc[4 * u + i] = sh.h.sc[e];
-          const uint8_t* vr = base + (int64_t)sh.h.pg[e] * a.cb + (int64_t)slot * a.cn + D + c * (DP / 16);
-#pragma unroll
-          for (int j = 0; j < KW; ++j)
-            b.v[4 * u + i][j] = c * (DP / 16) < D ? *reinterpret_cast<const uint32_t*>(vr + 4 * j) : 0u;
-        }
-      }
-    }
-  };
-
   auto compute = [&](int k0, Buf& b) {
     f32x4 sc[2];
 #pragma unroll
@@ -388,9 +427,12 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
                                                        qf[i], sc[u], 0, 0, 0);
     }
     float x[8], top = M0;
+    float2 ps[8];                              // the keys' scales
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ps[j] = sh.h.sc[b.e[j]];
     const bool edge = k0 < flo || k0 + 32 > fhi;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = sc[j / 4][j % 4] * (b.sc[j].x * rf);
+    for (int j = 0; j < 8; ++j) x[j] = sc[j / 4][j % 4] * (ps[j].x * rf);
     bool seen[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) seen[j] = true;
@@ -418,7 +460,7 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
     for (int j = 0; j < 8; ++j) {
       p[j] = __builtin_amdgcn_exp2f(x[j] - m + fbias);
       l += p[j];
-      p[j] *= b.sc[j].y;
+      p[j] *= ps[j].y;
     }
     if (edge) {
       // what no row sees may hold anything: as if it were zero
@@ -479,16 +521,13 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a, Split sp) {
     }
   };
 
-  Buf b0, b1;
-  int k = 32 * w;
-  if (k < nk) load(k, b0);
-  while (k < nk) {                             // 128 keys of the workgroup's four waves at a time, the next ones in flight
-    if (k + 128 < nk) load(k + 128, b1);
+  while (k < nk) {                             // 128 keys of the workgroup's four waves at a time, the next 128 in flight
     compute(k, b0);
+    if (k + 256 < nk) load(k + 256, b0);
     k += 128;
     if (k >= nk) break;
-    if (k + 128 < nk) load(k + 128, b0);
     compute(k, b1);
+    if (k + 256 < nk) load(k + 256, b1);
     k += 128;
   }
 
@@ -1067,20 +1106,22 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   }
 }
 
-// The parts joined, in their order: a wave for each (token, head), whose parts' weights lie over the lanes.  `all`: every
-// token of the call; else those of the requests that kv_attend_rows takes beside chunks.
+// Lanes that join a row: 4 elements each, a power of two.
+__host__ __device__ constexpr int join_lanes(int D) { return D <= 64 ? 16 : D <= 128 ? 32 : 64; }
+
+// The parts joined, in their order: a wave for some heads of a token.  `all`: every token of the call; else those of the
+// requests that kv_attend_rows takes beside chunks.
 __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split rows, Split tiles, int all) {
-  const int lane = threadIdx.x & 63, D = a.D;
-  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = id / a.Hq;
-  const int head = (int)(id - k * a.Hq), hd = head % a.G;
+  const int lane = threadIdx.x & 63, D = a.D, LG = join_lanes(D), per = 64 / LG, waves = (a.Hq + per - 1) / per;
+  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = id / waves;
+  const int head = (int)(id - k * waves) * per + lane / LG, hd = head % a.G, d = 4 * (lane % LG);
   Tile t;
   Request rq;
-  int64_t token = k;
+  int64_t token = k, first;
   if (all) {
     if (token >= a.st.T) return;
-    t.r = sdc_request_of(a.st, token, 1, 0);
+    t.r = sdc_find_request(a.st, token, 1, 0, rq, first);
     if (t.r < 0 || t.r >= a.st.R) return;
-    rq = sdc_request(a.st, t.r);
     if (token >= rq.q1) return;
   } else {
     t.r = (int)(k / tiles.few);
@@ -1097,36 +1138,27 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split rows, 
   find_keys(a, sp, rq, t);
   if (t.nsp < 2) return;
   const int row = tok * sp.GB + hd - t.hb * sp.GB;
-  const int64_t first = sp.slots ? (int64_t)t.r * sp.slots : (int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r;
+  first = sp.slots ? (int64_t)t.r * sp.slots : (int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r;
   const int64_t tile = ((first + tt) * a.Hkv + t.hk) * sp.NHB + t.hb, size = (int64_t)sp.rows * (D + 2);
   const float* rec = sp.part + tile * sp.S * size;
-  float m = M0;
-  for (int s = lane; s < t.nsp; s += 64) m = fmaxf(m, rec[s * size + 2 * row]);
-  m = wave_max_f32_dpp(m);
-  float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  const bool on = 4 * lane < D;
-  for (int b = 0; b < t.nsp; b += 64) {
-    const int n = min(64, t.nsp - b);
-    float f = 0.f;
-    if (lane < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(rec + (b + lane) * size + 2 * row);
-      f = exp2f(ml.x - m);
-      l += f * ml.y;
-    }
-    const float* p = rec + b * size + 2 * sp.rows + row * D + 4 * (on ? lane : 0);
+  if (head >= a.Hq || d >= D) return;
+  const float* ml = rec + 2 * row;
+  const float* v = rec + 2 * sp.rows + row * D + d;
+  float m = M0, l = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
-      const f32x4 v = *reinterpret_cast<const f32x4*>(p + s * size);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fmaf(fs, v[i], x[i]);
-    }
+  for (int s = 0; s < t.nsp; ++s) m = fmaxf(m, ml[s * size]);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < t.nsp; ++s) {
+    const float f = __builtin_amdgcn_exp2f(ml[s * size] - m);
+    l = fmaf(f, ml[s * size + 1], l);
+    x += f * *reinterpret_cast<const f32x4*>(v + s * size);
   }
-  l = wave_sum_f32_dpp(l);
   const int64_t p = t.p0 + tok;
   const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-  if (on) write_out(a, token, head, 4 * lane, x, 4, any ? 1.f / l : 0.f);
-  if (a.lse && lane == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l)) * LN2 : NEG_INF;
+  const float y[4] = {x[0], x[1], x[2], x[3]};
+  write_out(a, token, head, d, y, 4, any ? 1.f / l : 0.f);
+  if (a.lse && d == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l)) * LN2 : NEG_INF;
 }
 
 // The tiles and parts of a call, from its sizes alone.
@@ -1150,7 +1182,7 @@ void cut(Split& sp, int64_t busy, int64_t want, int64_t least, int64_t keys, int
   const int64_t most = std::min<int64_t>(16384, std::max<int64_t>(128, (MAXP - 2) * N / 128 * 128));
   sp.C = (int)std::min(least, most);
   keys += 31;
-  const int64_t s = std::min(std::max<int64_t>(1, want / std::max<int64_t>(1, busy)), sdc_cdiv(keys, sp.C));
+  const int64_t s = std::min(want / std::max<int64_t>(1, busy), keys / sp.C);
   // (a tile's keys over S parts, rounded up to 128, must stay within `most`)
   sp.S = (int)std::max<int64_t>({1, s, sdc_cdiv(keys, most)});
 }
@@ -1160,6 +1192,10 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
   auto keys = [&](const Split& sp) { return window > 0 ? std::min(max_len, window + sp.TB) : max_len; };
   p.rows = split_of(ROWS, G, N);
   p.tiles = split_of(32 * tall_waves(D), G, N);
+  // One round of the workgroups that the registers leave room for: 64 sequences of 512-2048 tokens 38 us (in two parts each
+  // 45, in four 57), four of 100-131k tokens 184 us (two rounds 192, four 210).  Parts of fewer than 512 keys cost more to
+  // join than they save.
+  const int64_t resident = 256 * (D <= 64 ? 3 : D <= 128 ? 2 : 1);
   // more tokens than requests: some have a chunk
   p.tall = T > R && T > FEW * p.rows.TB;
   if (p.tall) {
@@ -1168,10 +1204,10 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
     p.tiles.tiles = (T / p.tiles.TB + R + 1) * Hkv * p.tiles.NHB;
     cut(p.tiles, (T / p.tiles.TB + 1) * Hkv * p.tiles.NHB, 512, 512, keys(p.tiles), N);
     p.rows.tiles = R * FEW * Hkv * p.rows.NHB;
-    cut(p.rows, R * Hkv * p.rows.NHB, 1024, 256, keys(p.rows), N);
+    cut(p.rows, R * Hkv * p.rows.NHB, resident, 512, keys(p.rows), N);
   } else {
     p.rows.tiles = (T / p.rows.TB + R + 1) * Hkv * p.rows.NHB;
-    cut(p.rows, std::min(T, T / p.rows.TB + R) * Hkv * p.rows.NHB, 1024, 256, keys(p.rows), N);
+    cut(p.rows, std::min(T, T / p.rows.TB + R) * Hkv * p.rows.NHB, resident, 512, keys(p.rows), N);
   }
   return p;
 }
@@ -1180,7 +1216,8 @@ int64_t part_bytes(const Split& sp, int64_t D) { return sp.S <= 1 ? 0 : sp.tiles
 int launch_join(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   if (p.rows.S == 1 && p.tiles.S <= 1) return SDC_OK;
   const bool all = !p.tall || p.tiles.S > 1;
-  const int64_t blocks = sdc_cdiv((all ? a.st.T : (int64_t)a.st.R * p.tiles.few) * a.Hq, 4);
+  const int64_t waves = sdc_cdiv(a.Hq, 64 / join_lanes(a.D));
+  const int64_t blocks = sdc_cdiv((all ? a.st.T : (int64_t)a.st.R * p.tiles.few) * waves, 4);
   if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
   if (blocks == 0) return SDC_OK;
   SdcProf prof("kv_attend_join", stream);

@@ -21,22 +21,6 @@ struct Request {
   int64_t q0, q1, len;
 };
 
-// The last r in 0 .. R with qsl[r] / B + C r <= j, by the whole wave (all lanes active, j uniform), and -1 if there is
-// none; R stands for the tokens past the last request (the padding of a captured step).  Work items of up to B tokens each are numbered so that no scan over the requests is needed: request r's
-// items start at qsl[r] / B + C r.  With C = 1 that leaves room for items of B tokens from the request's first on, with
-// C = 2 for items that begin at positions divisible by B.  Every lane reads its requests' starts at once.
-__device__ __forceinline__ int sdc_request_of(const PagedStep& s, int64_t j, int B, int C) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int b = 0; b <= s.R; b += 64) {
-    const int i = b + lane;
-    const bool le = i <= s.R && (int64_t)((uint32_t)s.qsl[i] / (uint32_t)B) + (int64_t)C * i <= j;
-    const int c = __popcll(__ballot(le));
-    n += c;
-    if (c < 64) break;
-  }
-  return n - 1;
-}
 __device__ __forceinline__ Request sdc_request(const PagedStep& s, int r) {
   Request q;
   q.r = r;
@@ -49,4 +33,40 @@ __device__ __forceinline__ Request sdc_request(const PagedStep& s, int r) {
   q.q1 = min(max((int64_t)s.qsl[r + 1], q.q0), s.T);
   q.len = max(s.lens[r], 0);
   return q;
+}
+
+// The last r in 0 .. R with qsl[r] / B + C r <= j, by the whole wave (all lanes active, j uniform), and -1 if there is
+// none; R stands for the tokens past the last request (the padding of a captured step).  Work items of up to B tokens each
+// are numbered so that no scan over the requests is needed: request r's items start at qsl[r] / B + C r.  With C = 1 that
+// leaves room for items of B tokens from the request's first on, with C = 2 for items that begin at positions divisible by
+// B.  Every lane reads its requests' starts and lengths at once, so that up to 63 requests cost one trip to memory.
+// first: the number of the request's first item.
+__device__ __forceinline__ int sdc_find_request(const PagedStep& s, int64_t j, int B, int C, Request& q, int64_t& first) {
+  const int lane = threadIdx.x & 63;
+  int n = 0, b = 0, c = 0;
+  int32_t start = 0, len = 0;
+  for (; b <= s.R; b += 64) {
+    const int i = b + lane;
+    start = i <= s.R ? s.qsl[i] : 0;
+    len = i < s.R ? s.lens[i] : 0;
+    const bool le = i <= s.R && (int64_t)((uint32_t)start / (uint32_t)B) + (int64_t)C * i <= j;
+    c = __popcll(__ballot(le));
+    n += c;
+    if (c < 64) break;
+  }
+  const int r = n - 1;
+  if (r < 0) return r;
+  if (c > 0 && c < 64) {
+    // the request, and the one after it, are among those just read
+    const int32_t at = __builtin_amdgcn_readlane(start, c - 1), to = __builtin_amdgcn_readlane(start, c);
+    q.r = r;
+    q.q0 = min(max((int64_t)at, (int64_t)0), s.T);
+    q.q1 = r >= s.R ? s.T : min(max((int64_t)to, q.q0), s.T);
+    q.len = r >= s.R ? 0 : max(__builtin_amdgcn_readlane(len, c - 1), 0);
+    first = (int64_t)((uint32_t)at / (uint32_t)B) + (int64_t)C * r;
+  } else {
+    q = sdc_request(s, r);
+    first = (int64_t)((uint32_t)s.qsl[r] / (uint32_t)B) + (int64_t)C * r;
+  }
+  return r;
 }
