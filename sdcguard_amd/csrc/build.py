@@ -3,7 +3,8 @@
     python -m sdcguard_amd.csrc.build          # or sdcguard_amd.csrc.build.build()
 
 Every source is compiled with hipcc for gfx950 only, packed-fp32 instructions disabled, then linked into
-sdcguard_amd/libsdcguard_hip.so, which sdcguard_amd._lib loads with ctypes.
+sdcguard_amd/libsdcguard_hip.so, which sdcguard_amd._lib loads with ctypes.  bind.cpp, host code against torch's headers,
+becomes the extension module sdcguard_amd/_bind.so.
 """
 from __future__ import annotations
 
@@ -13,10 +14,12 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 LIB = os.path.join(PKG, "libsdcguard_hip.so")
+BIND = os.path.join(PKG, "_bind.so")
 OBJDIR = os.path.join(PKG, "_build")
 ARCH = os.environ.get("SDCGUARD_HIP_ARCH", "gfx950")
 
@@ -46,11 +49,29 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _bind() -> None:
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(_hipcc())))
+    tmp = BIND + ".tmp"
+    # -D: what HIP's host headers ask of a compiler that is not hipcc
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
+           "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(rocm, "include"), os.path.join(HERE, "bind.cpp"),
+           "-o", tmp, "-L", os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on bind.cpp:\n{r.stderr[-6000:]}")
+    os.replace(tmp, BIND)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = sources()
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        bind = ex.submit(_bind)
         objs = list(ex.map(_compile, srcs))
+        bind.result()
     tmp = LIB + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
