@@ -76,10 +76,29 @@ __device__ __forceinline__ float value_of(uint32_t c) {
   else return (float)(int8_t)c;
 }
 
-// n (8 or 1) codes at p
+// Four codes of values that are finite and lie within the codes' range.
+template <int CT>
+__device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
+  if constexpr (CT == SDC_CACHE_E4M3) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, lo, true);
+  } else {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = (uint32_t)(int)rintf(x[i] * inv);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0C0C0400u), __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u),
+                                 0x05040100u);
+  }
+}
+
+// n (8 or 1) codes at p; plain: the values are finite, and so large at most that the scale, a power of two, holds them
 template <int CT, int UP>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float* x, const Divide& d) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* x, const Divide& d, bool plain) {
   if constexpr (UP == 8) {
+    if (plain) {
+      *reinterpret_cast<u32x2*>(p) = u32x2{codes4<CT>(x, d.inv), codes4<CT>(x + 4, d.inv)};
+      return;
+    }
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -115,11 +134,63 @@ __device__ __forceinline__ void finite_max(float x, float& amax, bool& bad) {
   else bad = true;
 }
 
+// A unit of a key and of its value into the slot's row.
+template <int DT, int CT, int UP>
+__device__ __forceinline__ void put(uint8_t* row, RopeUnit rk, RopeUnit rv, int D, const float* x, const float* y,
+                                    const Divide& dk, const Divide& dv, bool plain) {
+  if constexpr (CT == SDC_CACHE_16) {
+    typedef typename RopeElem<DT>::T E;
+    sdc_store_unit<DT, UP>((E*)row, 1, rk, D, x);
+    sdc_store_unit<DT, UP>((E*)row + D, 1, rv, D, y);
+  } else {
+    store_codes<CT, UP>(row + rk.c0, x, dk, plain);
+    if (UP == 8 || rk.c1 < D) store_codes<CT, UP>(row + rk.c1, x + UP, dk, plain);
+    store_codes<CT, UP>(row + D + rv.c0, y, dv, plain);
+    if (UP == 8 || rv.c1 < D) store_codes<CT, UP>(row + D + rv.c1, y + UP, dv, plain);
+  }
+}
+
+// A page's largest magnitudes, scales and old codes: from the largest finite magnitudes of the new keys and values (of the
+// whole wave) and whether any is not finite, the scales to write with.  ok, ov: the page's scales before.
+template <int CT, int UP>
+__device__ __forceinline__ void settle(const AppendArgs& a, uint8_t* base, float* sc, int s0, int n, float mk, float mv, bool bk,
+                                       bool bv, float ok, float ov, float& sk, float& sv) {
+  const int lane = threadIdx.x & 63, N = a.st.N, D = a.D;
+  sk = scale_for<CT>(mk);
+  sv = scale_for<CT>(mv);
+  if (CT == SDC_CACHE_I8 && bk) sk = __builtin_nanf("");
+  if (CT == SDC_CACHE_I8 && bv) sv = __builtin_nanf("");
+  if (s0 > 0) {
+    sk = sk > ok ? sk : (sk == sk ? ok : sk);                           // (a scale that is NaN stays)
+    sv = sv > ov ? sv : (sv == sv ? ov : sv);
+    const float rk = ok / sk, rv = ov / sv;
+    const bool gk = ok < sk, gv = ov < sv;
+    if (gk || gv) {
+      constexpr int C = UP == 8 ? 8 : 1;
+      const int nc = D / C;
+      for (int i = lane; i < (N - n) * nc; i += 64) {
+        int s = i / nc;
+        const int c = (i - s * nc) * C;
+        if (s >= s0) s += n;
+        uint8_t* p = base + (int64_t)s * a.cn + c;
+        if (gk) rescale<CT, UP>(p, rk);
+        if (gv) rescale<CT, UP>(p + D, rv);
+      }
+    }
+  }
+  if (lane == 0) {
+    sc[0] = sk;
+    sc[1] = sv;
+  }
+}
+
 template <int DT, int CT, int UP>
 __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int hg, float2* tab) {
   typedef typename RopeElem<DT>::T E;
   const PagedStep& st = a.st;
   const int N = st.N, D = a.D, tid = threadIdx.x, lane = tid & 63;
+  const int P = a.rot / 2, nu = sdc_units(D, UP);
+  const double turn = P ? a.turns[tid % P] : 0.0;                       // (on its way while the request is found)
   Request rq;
   int64_t first;
   const int r = sdc_find_request(st, item, N, 2, rq, first);
@@ -128,18 +199,96 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   const int64_t w = pos0 / N + (item - first);
   const int64_t lo = max(pos0, w * N), hi = min(rq.len, (w + 1) * N);
   if (lo >= hi || w >= st.W) return;
-  const int64_t page = st.bt[r * st.sbt + w];
-  if (page < 0 || page >= st.NB) return;
+  const int32_t page = st.bt[r * st.sbt + w];
   const int n = (int)(hi - lo), s0 = (int)(lo - w * N);
   const int64_t t0 = rq.q1 - rq.len + lo;
   const int h = hg * 4 + (tid >> 6);
   const bool live = h < a.Hkv;
-  const int P = a.rot / 2, nu = sdc_units(D, UP);
-  const int rows = P ? min(n, TAB / P) : n;                             // tokens whose angles are held at once
-  uint8_t* base = a.kv + page * a.cb + (live ? h : 0) * a.ch;
   const E* kp = (const E*)a.k + (live ? h : 0) * a.skh;
   const E* vp = (const E*)a.v + (live ? h : 0) * a.svh;
+  const int units = n * nu;
 
+  // Up to HELD units a lane stay in registers, all loads of keys and values on their way at once (a token of 64 sequences each:
+  // 6.6 us, 12 with the two passes below, which larger pages take).
+  constexpr int HELD = 2;
+  if (units <= 64 * HELD && n * P <= TAB) {
+    float x[HELD][2 * UP], y[HELD][2 * UP];
+    RopeUnit ru[HELD], rv[HELD];
+    int tok[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      const int i = lane + 64 * j;
+      const bool on = live && i < units;
+      tok[j] = on ? i / nu : -1;
+      const int t = on ? tok[j] : 0, u = on ? i - t * nu : 0;
+      ru[j] = sdc_unit<UP>(u, a.rot, a.inter);
+      rv[j] = sdc_unit<UP>(u, 0, 0);
+      if (on) {
+        sdc_load_unit<DT, UP>(kp + (t0 + t) * a.skt, a.skd, ru[j], D, x[j]);
+        sdc_load_unit<DT, UP>(vp + (t0 + t) * a.svt, a.svd, rv[j], D, y[j]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2 * UP; ++e) x[j][e] = y[j][e] = 0.f;
+      }
+    }
+    if (page < 0 || page >= st.NB) return;
+    uint8_t* base = a.kv + (int64_t)page * a.cb + (live ? h : 0) * a.ch;
+    float* sc = a.scales + (int64_t)page * a.sb + (live ? h : 0) * a.sh;
+    float ok = 0.f, ov = 0.f;
+    if (CT != SDC_CACHE_16 && s0 > 0) {
+      ok = sc[0];
+      ov = sc[1];
+    }
+    for (int i = tid; i < n * P; i += 256) {
+      const int t = i / P;
+      tab[i] = sdc_turn(position_of(a, t0 + t, lo + t), i < 256 || 256 % P == 0 ? turn : a.turns[i - t * P], a.m);
+    }
+    __syncthreads();
+    if (!live) return;
+    // the largest magnitudes as bits, of which those of infinities and NaN are the largest
+    uint32_t uk = 0, uv = 0;
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if (tok[j] >= 0) sdc_rotate_unit<UP>(x[j], ru[j], a.inter, tab + tok[j] * P);
+#pragma unroll
+      for (int e = 0; e < 2 * UP; ++e) {
+        uk = max(uk, __float_as_uint(x[j][e]) & 0x7FFFFFFFu);
+        uv = max(uv, __float_as_uint(y[j][e]) & 0x7FFFFFFFu);
+      }
+    }
+    float sk = 1.f, sv = 1.f;
+    bool plain = false;
+    if constexpr (CT != SDC_CACHE_16) {
+      uk = wave_max_u32_dpp(uk);
+      uv = wave_max_u32_dpp(uv);
+      float mk = __uint_as_float(uk), mv = __uint_as_float(uv);
+      bool bk = false, bv = false;
+      plain = max(uk, uv) < 0x7F800000u;
+      if (!plain) {
+        mk = mv = 0.f;
+#pragma unroll 1
+        for (int j = 0; j < HELD; ++j)
+#pragma unroll
+          for (int e = 0; e < 2 * UP; ++e) {
+            finite_max(j ? x[1][e] : x[0][e], mk, bk);
+            finite_max(j ? y[1][e] : y[0][e], mv, bv);
+          }
+        mk = wave_max_f32_dpp(mk);
+        mv = wave_max_f32_dpp(mv);
+      }
+      settle<CT, UP>(a, base, sc, s0, n, mk, mv, __any(bk), __any(bv), ok, ov, sk, sv);
+    }
+    const Divide dk(sk), dv(sv);
+    plain = plain && dk.pow2 && dv.pow2;
+#pragma unroll
+    for (int j = 0; j < HELD; ++j)
+      if (tok[j] >= 0) put<DT, CT, UP>(base + (int64_t)(s0 + tok[j]) * a.cn, ru[j], rv[j], D, x[j], y[j], dk, dv, plain);
+    return;
+  }
+
+  if (page < 0 || page >= st.NB) return;
+  const int rows = P ? min(n, TAB / P) : n;                             // tokens whose angles are held at once
+  uint8_t* base = a.kv + (int64_t)page * a.cb + (live ? h : 0) * a.ch;
   auto angles = [&](int first) {                                        // by the whole workgroup
     const int m = min(rows, n - first);
     __syncthreads();
@@ -181,36 +330,9 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
       }
     }
     if (live) {
-      mk = wave_max_f32_dpp(mk);
-      mv = wave_max_f32_dpp(mv);
-      sk = scale_for<CT>(mk);
-      sv = scale_for<CT>(mv);
-      if (CT == SDC_CACHE_I8 && __any(bk)) sk = __builtin_nanf("");
-      if (CT == SDC_CACHE_I8 && __any(bv)) sv = __builtin_nanf("");
-      float* sc = a.scales + page * a.sb + h * a.sh;
-      if (s0 > 0) {
-        const float ok = sc[0], ov = sc[1];
-        sk = sk > ok ? sk : (sk == sk ? ok : sk);                       // (a scale that is NaN stays)
-        sv = sv > ov ? sv : (sv == sv ? ov : sv);
-        const float rk = ok / sk, rv = ov / sv;
-        const bool gk = ok < sk, gv = ov < sv;
-        if (gk || gv) {
-          constexpr int C = UP == 8 ? 8 : 1;
-          const int nc = D / C;
-          for (int i = lane; i < (N - n) * nc; i += 64) {
-            int s = i / nc;
-            const int c = (i - s * nc) * C;
-            if (s >= s0) s += n;
-            uint8_t* p = base + (int64_t)s * a.cn + c;
-            if (gk) rescale<CT, UP>(p, rk);
-            if (gv) rescale<CT, UP>(p + D, rv);
-          }
-        }
-      }
-      if (lane == 0) {
-        sc[0] = sk;
-        sc[1] = sv;
-      }
+      float* sc = a.scales + (int64_t)page * a.sb + h * a.sh;
+      const float ok = s0 > 0 ? sc[0] : 0.f, ov = s0 > 0 ? sc[1] : 0.f;
+      settle<CT, UP>(a, base, sc, s0, n, wave_max_f32_dpp(mk), wave_max_f32_dpp(mv), __any(bk), __any(bv), ok, ov, sk, sv);
     }
   }
   const Divide dk(sk), dv(sv);
@@ -220,56 +342,68 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
       const int t = i / nu, u = i - t * nu;
       float x[2 * UP], y[2 * UP];
       const RopeUnit rk = key(first, t, u, x), rv = value(first, t, u, y);
-      uint8_t* row = base + (int64_t)(s0 + first + t) * a.cn;
-      if constexpr (CT == SDC_CACHE_16) {
-        sdc_store_unit<DT, UP>((E*)row, 1, rk, D, x);
-        sdc_store_unit<DT, UP>((E*)row + D, 1, rv, D, y);
-      } else {
-        store_codes<CT, UP>(row + rk.c0, x, dk);
-        if (UP == 8 || rk.c1 < D) store_codes<CT, UP>(row + rk.c1, x + UP, dk);
-        store_codes<CT, UP>(row + D + rv.c0, y, dv);
-        if (UP == 8 || rv.c1 < D) store_codes<CT, UP>(row + D + rv.c1, y + UP, dv);
-      }
+      put<DT, CT, UP>(base + (int64_t)(s0 + first + t) * a.cn, rk, rv, D, x, y, dk, dv, false);
     }
   }
 }
 
-// The queries of QTOK tokens, rotated; those past the last request are written as zeros.
+// The queries of QTOK tokens, rotated; those past the last request are written as zeros.  A thread's first unit is on its
+// way while the tokens' requests are found.
 template <int DT, int UP>
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t block, float2* tab) {
   typedef typename RopeElem<DT>::T E;
+  constexpr int HELD = 1;
   const int tid = threadIdx.x, P = a.rot / 2, nu = sdc_units(a.D, UP);
   const int TB = P ? min(QTOK, TAB / P) : QTOK;
   __shared__ int64_t own[QTOK];                                         // the tokens' positions in their requests
   for (int64_t t0 = block * QTOK, te = min(t0 + QTOK, a.st.T); t0 < te; t0 += TB) {
-    const int nt = (int)min((int64_t)TB, te - t0);
+    const int nt = (int)min((int64_t)TB, te - t0), all = nt * a.Hq * nu;
+    struct Unit {
+      int t, h;
+      RopeUnit ru;
+      float x[2 * UP];
+    };
+    auto load = [&](int i, Unit& u) {
+      const int th = i / nu;
+      u.t = th / a.Hq;
+      u.h = th - u.t * a.Hq;
+      u.ru = sdc_unit<UP>(i - th * nu, a.rot, a.inter);
+      sdc_load_unit<DT, UP>((const E*)a.q + (t0 + u.t) * a.sqt + u.h * a.sqh, a.sqd, u.ru, a.D, u.x);
+    };
+    auto store = [&](Unit& u) {
+      sdc_rotate_unit<UP>(u.x, u.ru, a.inter, tab + u.t * P);
+      if (own[u.t] < 0) {
+#pragma unroll
+        for (int e = 0; e < 2 * UP; ++e) u.x[e] = 0.f;
+      }
+      sdc_store_unit<DT, UP>((E*)a.qo + (t0 + u.t) * a.sot + u.h * a.soh, a.sod, u.ru, a.D, u.x);
+    };
+    const double turn = P && tid < nt * P ? a.turns[tid % P] : 0.0;
+    Unit held[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j)
+      if (tid + 256 * j < all) load(tid + 256 * j, held[j]);
     __syncthreads();
     for (int t = tid >> 6; t < nt; t += 4) {                            // a wave per token: its request, its position
       Request rq;
       int64_t first, p = -1;
       const int r = sdc_find_request(a.st, t0 + t, 1, 0, rq, first);
-      if (r >= 0 && r < a.st.R) {
-        p = max(t0 + t - rq.q1 + rq.len, (int64_t)0);
-      }
+      if (r >= 0 && r < a.st.R) p = max(t0 + t - rq.q1 + rq.len, (int64_t)0);
       if ((tid & 63) == 0) own[t] = p;
     }
     __syncthreads();
     for (int i = tid; i < nt * P; i += 256) {
       const int t = i / P;
-      tab[i] = sdc_turn(position_of(a, t0 + t, own[t]), a.turns[i - t * P], a.m);
+      tab[i] = sdc_turn(position_of(a, t0 + t, own[t]), i < 256 || 256 % P == 0 ? turn : a.turns[i - t * P], a.m);
     }
     __syncthreads();
-    for (int i = tid; i < nt * a.Hq * nu; i += 256) {
-      const int th = i / nu, u = i - th * nu, t = th / a.Hq, h = th - t * a.Hq;
-      const RopeUnit ru = sdc_unit<UP>(u, a.rot, a.inter);
-      float x[2 * UP];
-      sdc_load_unit<DT, UP>((const E*)a.q + (t0 + t) * a.sqt + h * a.sqh, a.sqd, ru, a.D, x);
-      sdc_rotate_unit<UP>(x, ru, a.inter, tab + t * P);
-      if (own[t] < 0) {
 #pragma unroll
-        for (int e = 0; e < 2 * UP; ++e) x[e] = 0.f;
-      }
-      sdc_store_unit<DT, UP>((E*)a.qo + (t0 + t) * a.sot + h * a.soh, a.sod, ru, a.D, x);
+    for (int j = 0; j < HELD; ++j)
+      if (tid + 256 * j < all) store(held[j]);
+    for (int i = tid + 256 * HELD; i < all; i += 256) {
+      Unit u;
+      load(i, u);
+      store(u);
     }
   }
 }
@@ -281,7 +415,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   if (b < pages) append_page<DT, CT, UP>(a, (int)(b / a.hgroups), (int)(b % a.hgroups), tab);
   else rotate_queries<DT, UP>(a, b - pages, tab);
 }
-
 template <int DT, int CT, int UP>
 int launch(const AppendArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.items * a.hgroups + (a.q ? sdc_cdiv(a.st.T, QTOK) : 0);

@@ -39,30 +39,38 @@ __device__ __forceinline__ Request sdc_request(const PagedStep& s, int r) {
 // none; R stands for the tokens past the last request (the padding of a captured step).  Work items of up to B tokens each
 // are numbered so that no scan over the requests is needed: request r's items start at qsl[r] / B + C r.  With C = 1 that
 // leaves room for items of B tokens from the request's first on, with C = 2 for items that begin at positions divisible by
-// B.  Every lane reads its requests' starts and lengths at once, so that up to 63 requests cost one trip to memory.
+// B.  Every lane reads two requests' starts and lengths at once, so that up to 127 requests cost one trip to memory.
 // first: the number of the request's first item.
 __device__ __forceinline__ int sdc_find_request(const PagedStep& s, int64_t j, int B, int C, Request& q, int64_t& first) {
   const int lane = threadIdx.x & 63;
-  int n = 0, b = 0, c = 0;
-  int32_t start = 0, len = 0;
-  for (; b <= s.R; b += 64) {
-    const int i = b + lane;
-    start = i <= s.R ? s.qsl[i] : 0;
-    len = i < s.R ? s.lens[i] : 0;
-    const bool le = i <= s.R && (int64_t)((uint32_t)start / (uint32_t)B) + (int64_t)C * i <= j;
-    c = __popcll(__ballot(le));
+  int n = 0, c = 0;
+  int32_t start[2] = {0, 0}, len[2] = {0, 0};
+  for (int b = 0; b <= s.R; b += 128) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = min(b + 64 * u + lane, s.R);
+      start[u] = s.qsl[i];
+      len[u] = s.R ? s.lens[min(i, s.R - 1)] : 0;
+    }
+    c = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = b + 64 * u + lane;
+      c += __popcll(__ballot(i <= s.R && (int64_t)((uint32_t)start[u] / (uint32_t)B) + (int64_t)C * i <= j));
+    }
     n += c;
-    if (c < 64) break;
+    if (c < 128) break;
   }
   const int r = n - 1;
   if (r < 0) return r;
-  if (c > 0 && c < 64) {
+  if (c > 0 && c < 128) {
     // the request, and the one after it, are among those just read
-    const int32_t at = __builtin_amdgcn_readlane(start, c - 1), to = __builtin_amdgcn_readlane(start, c);
+    const int32_t at = __builtin_amdgcn_readlane(c > 64 ? start[1] : start[0], (c - 1) & 63);
+    const int32_t to = __builtin_amdgcn_readlane(c > 63 ? start[1] : start[0], c & 63);
     q.r = r;
     q.q0 = min(max((int64_t)at, (int64_t)0), s.T);
     q.q1 = r >= s.R ? s.T : min(max((int64_t)to, q.q0), s.T);
-    q.len = r >= s.R ? 0 : max(__builtin_amdgcn_readlane(len, c - 1), 0);
+    q.len = r >= s.R ? 0 : max(__builtin_amdgcn_readlane(c > 64 ? len[1] : len[0], (c - 1) & 63), 0);
     first = (int64_t)((uint32_t)at / (uint32_t)B) + (int64_t)C * r;
   } else {
     q = sdc_request(s, r);
