@@ -206,6 +206,20 @@ __device__ __forceinline__ bool find_tile(const AttendArgs& a, const Split& sp, 
   return true;
 }
 
+// Four results of a row at element d (a multiple of 4), scaled.
+__device__ __forceinline__ void write_four(const AttendArgs& a, int64_t tok, int h, int d, f32x4 x, float f) {
+  uint16_t* o = a.o + tok * a.sot + h * a.soh;
+  x *= f;
+  uint32_t v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    v[i] = a.fp16 ? sdc_to_half<SDC_FP16>(x[2 * i]) | (uint32_t)sdc_to_half<SDC_FP16>(x[2 * i + 1]) << 16
+                  : sdc_to_half<SDC_BF16>(x[2 * i]) | (uint32_t)sdc_to_half<SDC_BF16>(x[2 * i + 1]) << 16;
+  if (a.sod == 1 && ((uintptr_t)a.o % 8 | (uint64_t)(a.sot | a.soh) % 4) == 0) *reinterpret_cast<u32x2*>(o + d) = u32x2{v[0], v[1]};
+  else
+    for (int i = 0; i < 4; ++i) o[(d + i) * a.sod] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+}
+
 // One row's results: x[0 .. n) at elements d.., scaled.
 __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t tok, int h, int d, const float* x, int n, float f) {
   uint16_t* o = a.o + tok * a.sot + h * a.soh;
@@ -221,8 +235,12 @@ __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t tok, int 
 // fp16; queries are scaled to it by a power of two per row (a bf16 element 2^-27 of its row's largest keeps all bits).
 // The key scales multiply the scores, the value scales the probabilities, in fp32.  Probabilities are rounded to fp16's
 // 11 bits, in units that put their largest product with a value scale at 2^13 .. 2^15.
+// Waves of a workgroup, which a lane's registers leave room for.
+constexpr int row_waves(int D) { return D > 128 ? 4 : 8; }
+
 template <int CT, int DP, int PN>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendArgs a, Split sp) {
+__global__ __launch_bounds__(64 * row_waves(DP), row_waves(DP) / 4) void kv_attend_rows(AttendArgs a, Split sp) {
+  constexpr int NW = row_waves(DP), KEYS = 32 * NW;                     // keys that the workgroup's waves take at a time
   constexpr int KW = DP / 64;                  // 16-byte reads of a key per lane; dwords of a value per lane
   constexpr int NS = DP / 32, ND = DP / 16;    // depth steps of a score, row blocks of the output
   constexpr int QS = DP + 8, OS = DP + 4;      // row pitches in LDS
@@ -233,18 +251,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
   };
   __shared__ union {
     Head h;
-    float o[4][ROWS][OS];
+    float o[NW][ROWS][OS];
   } sh;
-  __shared__ float rowf[ROWS], wmax[4], ml[4][ROWS][2];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
+  __shared__ float rowf[ROWS], wmax[NW], ml[NW][ROWS][2];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = a.D, N = a.st.N;
   const int s = blockIdx.x % sp.S, tile = blockIdx.x / sp.S;
   Tile t;
   if (!find_tile(a, sp, tile, t)) return;
   if (s >= max(t.nsp, 1)) return;
-  const int orow = tid >> 4, od = (tid & 15) * ND;                      // the output a thread writes: row, elements
+  const int orow = (tid >> 4) & 15, od = (tid & 15) * ND;               // the output that a thread of the first 256 writes
   const int otok = orow / sp.GB, oh = t.hb * sp.GB + orow % sp.GB;
-  const bool olive = orow < sp.GB * sp.TB && otok < t.ntok && oh < a.G;
+  const bool olive = tid < 256 && orow < sp.GB * sp.TB && otok < t.ntok && oh < a.G;
   const int64_t otoken = t.tok0 + otok;
   const int ohead = t.hk * a.G + oh;
   if (t.nsp == 0) {                            // no row sees a key
@@ -260,7 +279,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
   const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
 
   // the part's pages; a page outside the cache is page 0, marked by its sign
-  for (int i = tid; i < np; i += 256) {
+  for (int i = tid; i < np; i += 64 * NW) {
     const int32_t page = a.st.bt[t.r * a.st.sbt + fp + i];
     sh.h.pg[i] = page >= 0 && page < a.st.NB ? page : (int32_t)0x80000000;
   }
@@ -294,7 +313,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
   // page entry and slot of a key counted from a0
   auto place = [&](int key, int& slot) {
     const uint32_t loc = (uint32_t)(base0 + key);
-    const int i = N == 1 ? (int)loc : (int)__umulhi(loc, sp.div);
+    const int i = PN == 1 && N == 1 ? (int)loc : (int)__umulhi(loc, sp.div);
     slot = (int)loc - i * N;
     return min(i, np - 1);
   };
@@ -303,60 +322,65 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
     uint32_t v[8][KW];
     int e[8];                                  // the keys' page entries
   };
+  // where a lane's codes lie in its rows; columns past the head's are read from its last ones (keys': then taken as zeros)
+  const uint32_t cn = (uint32_t)a.cn;          // (N cn is below 2^31)
+  uint32_t kcol[KW];
+#pragma unroll
+  for (int j = 0; j < KW; ++j) kcol[j] = min(g * (DP / 4) + 16 * j, D - 16);
+  const uint32_t vcol = D + min(c * (DP / 16), D - DP / 16);
+  const uint32_t krow = c * cn, vrow = 4 * g * cn + vcol;
+  typedef uint32_t vt __attribute__((ext_vector_type(KW)));
   auto load = [&](int k0, Buf& b) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      int slot, e;
-      const uint8_t* row;
+      int slot;
       if constexpr (PN == 16) {                // the 16 keys lie in one page
-        e = __builtin_amdgcn_readfirstlane(place(k0 + 16 * u, slot));
-        slot = __builtin_amdgcn_readfirstlane(slot);
-        row = base + (int64_t)(__builtin_amdgcn_readfirstlane(sh.h.pg[e]) & 0x7FFFFFFF) * a.cb + (int64_t)slot * a.cn;
-        const uint8_t* kr = row + c * a.cn + g * (DP / 4);
+        const int e = place(__builtin_amdgcn_readfirstlane(k0 + 16 * u), slot);
+        const uint8_t* row = base + (int64_t)(__builtin_amdgcn_readfirstlane(sh.h.pg[e]) & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
 #pragma unroll
-        for (int j = 0; j < KW; ++j)
-          b.k[u][j] = g * (DP / 4) + 16 * j < D ? *reinterpret_cast<const u32x4*>(kr + 16 * j) : u32x4{0, 0, 0, 0};
+        for (int j = 0; j < KW; ++j) b.k[u][j] = *reinterpret_cast<const u32x4*>(row + (krow + kcol[j]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* vr = row + (4 * g + i) * a.cn + D + c * (DP / 16);
+          vt x;
+          if constexpr (KW == 1) x[0] = *reinterpret_cast<const uint32_t*>(row + i * cn + vrow);
+          else x = *reinterpret_cast<const vt*>(row + i * cn + vrow);
           b.e[4 * u + i] = e;
-          typedef uint32_t vt __attribute__((ext_vector_type(KW)));
-          if constexpr (KW == 1) b.v[4 * u + i][0] = c * (DP / 16) < D ? *reinterpret_cast<const uint32_t*>(vr) : 0u;
-          else {
-            vt x = {};
-            if (c * (DP / 16) < D) x = *reinterpret_cast<const vt*>(vr);
 #pragma unroll
-            for (int j = 0; j < KW; ++j) b.v[4 * u + i][j] = x[j];
-          }
+          for (int j = 0; j < KW; ++j) b.v[4 * u + i][j] = x[j];
         }
       } else {
-        e = place(k0 + 16 * u + c, slot);
-        row = base + (int64_t)(sh.h.pg[e] & 0x7FFFFFFF) * a.cb + (int64_t)slot * a.cn;
+        int e = place(k0 + 16 * u + c, slot);
+        const uint8_t* row = base + (int64_t)(sh.h.pg[e] & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn;
 #pragma unroll
-        for (int j = 0; j < KW; ++j)
-          b.k[u][j] = g * (DP / 4) + 16 * j < D ? *reinterpret_cast<const u32x4*>(row + g * (DP / 4) + 16 * j) : u32x4{0, 0, 0, 0};
+        for (int j = 0; j < KW; ++j) b.k[u][j] = *reinterpret_cast<const u32x4*>(row + kcol[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           e = place(k0 + 16 * u + 4 * g + i, slot);
           b.e[4 * u + i] = e;
-          const uint8_t* vr = base + (int64_t)(sh.h.pg[e] & 0x7FFFFFFF) * a.cb + (int64_t)slot * a.cn + D + c * (DP / 16);
+          const uint8_t* vr = base + (int64_t)(sh.h.pg[e] & 0x7FFFFFFF) * a.cb + (uint32_t)slot * cn + vcol;
 #pragma unroll
-          for (int j = 0; j < KW; ++j)
-            b.v[4 * u + i][j] = c * (DP / 16) < D ? *reinterpret_cast<const uint32_t*>(vr + 4 * j) : 0u;
+          for (int j = 0; j < KW; ++j) b.v[4 * u + i][j] = *reinterpret_cast<const uint32_t*>(vr + 4 * j);
         }
       }
     }
   };
 
+  // the pages' scales, then the first codes: a wait for the former leaves the latter on their way
+  float vmax = 0.f;
   Buf b0, b1;
   int k = 32 * w;
-  if (k < nk) load(k, b0);                     // (on their way while the scales are read and the queries put in place)
-  if (k + 128 < nk) load(k + 128, b1);
-  float vmax = 0.f;
-  for (int i = tid; i < np; i += 256) {
+  float2 sc0 = {0.f, 0.f};
+  if (tid < np) {
+    const float* scp = a.scales + (int64_t)(sh.h.pg[tid] & 0x7FFFFFFF) * a.sb + t.hk * a.sh;
+    sc0 = {scp[0], scp[1]};
+  }
+  if (k < nk) load(k, b0);
+  if (k + KEYS < nk) load(k + KEYS, b1);
+  for (int i = tid; i < np; i += 64 * NW) {
     const int32_t page = sh.h.pg[i];
     const float* scp = a.scales + (int64_t)(page & 0x7FFFFFFF) * a.sb + t.hk * a.sh;
-    float2 sc = {scp[0], scp[1]};
+    float2 sc = sc0;
+    if (i != tid) sc = {scp[0], scp[1]};
     if (page < 0) sc = {__builtin_nanf(""), __builtin_nanf("")};
     sh.h.sc[i] = sc;
     const float v = fabsf(sc.y);
@@ -389,13 +413,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
     e = max(e, -100);
     const float f = ldexpf(1.f, 13 - e);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) sh.h.q[orow][od + i] = (_Float16)(x[i] * f);
-    if ((tid & 15) == 0) rowf[orow] = ldexpf(a.scale, e - 13);
+    for (int i = 0; i < ND; ++i)
+      if (tid < 256) sh.h.q[orow][od + i] = (_Float16)(x[i] * f);
+    if (tid < 256 && (tid & 15) == 0) rowf[orow] = ldexpf(a.scale, e - 13);
   }
   vmax = wave_max_f32_dpp(vmax);
   if (lane == 0) wmax[w] = vmax;
   __syncthreads();
-  vmax = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+#pragma unroll
+  for (int i = 0; i < NW; ++i) vmax = fmaxf(vmax, wmax[i]);
   int ve;
   (void)frexpf(vmax, &ve);
   const int bias = 13 - min(max(ve, -100), 100);                        // probabilities in units of 2^-bias
@@ -417,6 +443,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
   for (int n = 0; n < ND; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = M0, l = 0.f;
   auto compute = [&](int k0, Buf& b) {
+    if (D < DP) {
+      asm volatile("");                        // (a branch)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < KW; ++j)
+          if (g * (DP / 4) + 16 * j >= D) b.k[u][j] = u32x4{0, 0, 0, 0};
+    }
     f32x4 sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -521,17 +555,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
     }
   };
 
-  while (k < nk) {                             // 128 keys of the workgroup's four waves at a time, the next 128 in flight
+  while (k < nk) {                             // the next keys in flight
     compute(k, b0);
-    if (k + 256 < nk) load(k + 256, b0);
-    k += 128;
+    if (k + 2 * KEYS < nk) load(k + 2 * KEYS, b0);
+    k += KEYS;
     if (k >= nk) break;
     compute(k, b1);
-    if (k + 256 < nk) load(k + 256, b1);
-    k += 128;
+    if (k + 2 * KEYS < nk) load(k + 2 * KEYS, b1);
+    k += KEYS;
   }
 
-  // the four waves' sums joined: a lane holds DP / 4 adjacent outputs of its row
+  // the waves' sums joined: a lane holds DP / 4 adjacent outputs of its row
   l = over_groups_sum(l);
   __syncthreads();
   if (g == 0) {
@@ -544,35 +578,36 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
     for (int n = 0; n < ND; n += 4)
       *reinterpret_cast<f32x4*>(&sh.o[w][c][(4 * g + i) * ND + n]) = f32x4{o[n][i], o[n + 1][i], o[n + 2][i], o[n + 3][i]};
   __syncthreads();
-  float mt = M0, lt = 0.f, f[4];
+  constexpr int Q = DP / 4;                    // threads of a row, four elements each
+  for (int i = tid; i < ROWS * Q; i += 64 * NW) {
+    const int row = i / Q, d = 4 * (i - row * Q), tok = row / sp.GB, hd = t.hb * sp.GB + row % sp.GB;
+    if (row >= sp.GB * sp.TB || tok >= t.ntok || hd >= a.G || d >= D) continue;
+    const int64_t token = t.tok0 + tok;
+    const int head = t.hk * a.G + hd;
+    float mt = M0, lt = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mt = fmaxf(mt, ml[i][orow][0]);
+    for (int u = 0; u < NW; ++u) mt = fmaxf(mt, ml[u][row][0]);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = exp2f(ml[i][orow][0] - mt);
-    lt += f[i] * ml[i][orow][1];
-  }
-  float x[ND];
-#pragma unroll
-  for (int n = 0; n < ND; ++n) {
-    x[n] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[n] += f[i] * sh.o[i][orow][od + n];
-  }
-  if (!olive) return;
-  if (t.nsp == 1) {
-    // (a row with keys whose scores are all -inf: 0 / 0)
-    const int64_t p = t.p0 + otok;
-    const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-    write_out(a, otoken, ohead, od, x, ND, any ? 1.f / lt : 0.f);
-    if (a.lse && (tid & 15) == 0) a.lse[otoken * a.slt + ohead] = any ? (mt + log2f(lt) - fbias) * LN2 : NEG_INF;
-  } else {
-    float* rec = sp.part + (int64_t)blockIdx.x * ROWS * (D + 2);
-    if ((tid & 15) == 0) {
-      rec[2 * orow] = mt;
-      rec[2 * orow + 1] = lt * unit;
+    for (int u = 0; u < NW; ++u) {
+      const float f = __builtin_amdgcn_exp2f(ml[u][row][0] - mt);
+      lt = fmaf(f, ml[u][row][1], lt);
+      x += f * *reinterpret_cast<const f32x4*>(&sh.o[u][row][d]);
     }
-    for (int n = 0; n < ND && od + n < D; ++n) rec[2 * ROWS + orow * D + od + n] = x[n] * unit;
+    if (t.nsp == 1) {
+      // (a row with keys whose scores are all -inf: 0 / 0)
+      const int64_t p = t.p0 + tok;
+      const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
+      write_four(a, token, head, d, x, any ? 1.f / lt : 0.f);
+      if (a.lse && d == 0) a.lse[token * a.slt + head] = any ? (mt + log2f(lt) - fbias) * LN2 : NEG_INF;
+    } else {
+      float* rec = sp.part + (int64_t)blockIdx.x * ROWS * (D + 2);
+      if (d == 0) {
+        rec[2 * row] = mt;
+        rec[2 * row + 1] = lt * unit;
+      }
+      *reinterpret_cast<f32x4*>(rec + 2 * ROWS + row * D + d) = x * unit;
+    }
   }
 }
 
@@ -647,25 +682,10 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     r.head = t.hk * a.G + (r.live ? hd : 0);
     return r;
   };
-  auto put = [&](const Row& r, int d, float x0, float x1, float x2, float x3) {        // four results at element d
-    uint16_t* op = a.o + r.token * a.sot + r.head * a.soh;
-    const bool wide = a.sod == 1 && ((uintptr_t)a.o % 8 | (uint64_t)(a.sot | a.soh) % 4) == 0;
-    uint32_t v[2];
-    if (a.fp16) {
-      v[0] = sdc_to_half<SDC_FP16>(x0) | (uint32_t)sdc_to_half<SDC_FP16>(x1) << 16;
-      v[1] = sdc_to_half<SDC_FP16>(x2) | (uint32_t)sdc_to_half<SDC_FP16>(x3) << 16;
-    } else {
-      v[0] = sdc_to_half<SDC_BF16>(x0) | (uint32_t)sdc_to_half<SDC_BF16>(x1) << 16;
-      v[1] = sdc_to_half<SDC_BF16>(x2) | (uint32_t)sdc_to_half<SDC_BF16>(x3) << 16;
-    }
-    if (wide) *reinterpret_cast<u32x2*>(op + d) = u32x2{v[0], v[1]};
-    else
-      for (int i = 0; i < 4; ++i) op[(d + i) * a.sod] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
-  };
   if (t.nsp == 0) {                            // no row sees a key
     const Row r = row_of();
     if (r.live) {
-      for (int d = 4 * h; d < D; d += 8) put(r, d, 0.f, 0.f, 0.f, 0.f);
+      for (int d = 4 * h; d < D; d += 8) write_four(a, r.token, r.head, d, f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
       if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = NEG_INF;
     }
     return;
@@ -1087,10 +1107,10 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     // (a row with keys whose scores are all -inf: 0 / 0)
     const int64_t p = t.p0 + r.tok;
     const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-    const float f = 1.f / l;
+    const float f = any ? 1.f / l : 0.f;
     each([&](int d, f32x4 x) {
-      if (d < D) put(r, d, any ? x[0] * f : 0.f, any ? x[1] * f : 0.f, any ? x[2] * f : 0.f, any ? x[3] * f : 0.f);
-    }, [&](int d, float x) { write_out(a, r.token, r.head, d, &x, 1, any ? f : 0.f); });
+      if (d < D) write_four(a, r.token, r.head, d, x, f);
+    }, [&](int d, float x) { write_out(a, r.token, r.head, d, &x, 1, f); });
     if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = any ? (m + log2f(l) - BIAS) * LN2 : NEG_INF;
   } else {
     float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + 2);
@@ -1156,8 +1176,7 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split rows, 
   }
   const int64_t p = t.p0 + tok;
   const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-  const float y[4] = {x[0], x[1], x[2], x[3]};
-  write_out(a, token, head, d, y, 4, any ? 1.f / l : 0.f);
+  write_four(a, token, head, d, x, any ? 1.f / l : 0.f);
   if (a.lse && d == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l)) * LN2 : NEG_INF;
 }
 
@@ -1192,10 +1211,10 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
   auto keys = [&](const Split& sp) { return window > 0 ? std::min(max_len, window + sp.TB) : max_len; };
   p.rows = split_of(ROWS, G, N);
   p.tiles = split_of(32 * tall_waves(D), G, N);
-  // One round of the workgroups that the registers leave room for: 64 sequences of 512-2048 tokens 38 us (in two parts each
-  // 45, in four 57), four of 100-131k tokens 184 us (two rounds 192, four 210).  Parts of fewer than 512 keys cost more to
-  // join than they save.
-  const int64_t resident = 256 * (D <= 64 ? 3 : D <= 128 ? 2 : 1);
+  // One round of the workgroups that the registers leave room for, one a CU: with two and three rounds 32 sequences of
+  // 1000-4000 tokens take 49 and 57 us (44), four of 100-131k tokens 185 and 192 (186).  Parts of fewer than 512 keys cost
+  // more to join than they save.
+  constexpr int64_t resident = 256;
   // more tokens than requests: some have a chunk
   p.tall = T > R && T > FEW * p.rows.TB;
   if (p.tall) {
@@ -1231,10 +1250,9 @@ int launch_rows(const AttendArgs& a, const Split& sp, hipStream_t stream) {
   if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
   if (blocks == 0) return SDC_OK;
   SdcProf prof("kv_attend", stream);
-  if (a.st.N % 16 == 0)
-    hipLaunchKernelGGL((kv_attend_rows<CT, DP, 16>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sp);
-  else
-    hipLaunchKernelGGL((kv_attend_rows<CT, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, a, sp);
+  const dim3 grid((unsigned)blocks), threads(64 * row_waves(DP));
+  if (a.st.N % 16 == 0) hipLaunchKernelGGL((kv_attend_rows<CT, DP, 16>), grid, threads, 0, stream, a, sp);
+  else hipLaunchKernelGGL((kv_attend_rows<CT, DP, 1>), grid, threads, 0, stream, a, sp);
   SDC_LAUNCH_CHECK();
   return SDC_OK;
 }
