@@ -235,12 +235,9 @@ __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t tok, int 
 // fp16; queries are scaled to it by a power of two per row (a bf16 element 2^-27 of its row's largest keeps all bits).
 // The key scales multiply the scores, the value scales the probabilities, in fp32.  Probabilities are rounded to fp16's
 // 11 bits, in units that put their largest product with a value scale at 2^13 .. 2^15.
-// Waves of a workgroup, which a lane's registers leave room for.
-constexpr int row_waves(int D) { return D > 128 ? 4 : 8; }
-
 template <int CT, int DP, int PN>
-__global__ __launch_bounds__(64 * row_waves(DP), row_waves(DP) / 4) void kv_attend_rows(AttendArgs a, Split sp) {
-  constexpr int NW = row_waves(DP), KEYS = 32 * NW;                     // keys that the workgroup's waves take at a time
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendArgs a, Split sp) {
+  constexpr int NW = 4, KEYS = 32 * NW;                     // keys that the workgroup's waves take at a time
   constexpr int KW = DP / 64;                  // 16-byte reads of a key per lane; dwords of a value per lane
   constexpr int NS = DP / 32, ND = DP / 16;    // depth steps of a score, row blocks of the output
   constexpr int QS = DP + 8, OS = DP + 4;      // row pitches in LDS
@@ -946,7 +943,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   // the softmax and the values' products of a tile whose scores are x; between its exponentials, the next tile's scores
   auto finish = [&](int k0, const Stage& d, f32x16* x, const uint8_t* next, f32x16* y) {
     // Fragments are read AHEAD products before they are used (left to itself the compiler reads one at a time and waits for
-    // it: 320 us instead of XXX), first the keys', then the values', neighbours into different accumulators.
+    // it: two prompt chunks of 2048 tokens 323 us, 297 so), first the keys', then the values', neighbours into different accumulators.
     constexpr int MK = KB * NS, MV = ND * KT / 16, AHEAD = 4;
     f16x8 fr[AHEAD];
     auto fragment = [&](int q) {
@@ -1211,10 +1208,10 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
   auto keys = [&](const Split& sp) { return window > 0 ? std::min(max_len, window + sp.TB) : max_len; };
   p.rows = split_of(ROWS, G, N);
   p.tiles = split_of(32 * tall_waves(D), G, N);
-  // One round of the workgroups that the registers leave room for, one a CU: with two and three rounds 32 sequences of
-  // 1000-4000 tokens take 49 and 57 us (44), four of 100-131k tokens 185 and 192 (186).  Parts of fewer than 512 keys cost
-  // more to join than they save.
-  constexpr int64_t resident = 256;
+  // One round of the workgroups that a lane's registers leave room for, two a CU: 64 sequences of 512-2048 tokens 34.5 us,
+  // four of 100-131k 179 us, 32 of 1000-4000 with their append 44 us (three rounds: 34.5, 184 and 45).  Parts of fewer than 512
+  // keys cost more to join than they save.  (Workgroups of eight waves, one a CU: 41, 182 and 42.)
+  constexpr int64_t resident = 512;
   // more tokens than requests: some have a chunk
   p.tall = T > R && T > FEW * p.rows.TB;
   if (p.tall) {
@@ -1250,7 +1247,7 @@ int launch_rows(const AttendArgs& a, const Split& sp, hipStream_t stream) {
   if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
   if (blocks == 0) return SDC_OK;
   SdcProf prof("kv_attend", stream);
-  const dim3 grid((unsigned)blocks), threads(64 * row_waves(DP));
+  const dim3 grid((unsigned)blocks), threads(256);
   if (a.st.N % 16 == 0) hipLaunchKernelGGL((kv_attend_rows<CT, DP, 16>), grid, threads, 0, stream, a, sp);
   else hipLaunchKernelGGL((kv_attend_rows<CT, DP, 1>), grid, threads, 0, stream, a, sp);
   SDC_LAUNCH_CHECK();
