@@ -13,6 +13,8 @@
 // are not finite take no part in the scale; e4m3 keeps them as NaN, int8, which has no such code, makes the scale NaN.
 #include <float.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "paged.h"
 #include "profile.h"
@@ -35,6 +37,7 @@ struct AppendArgs {
   const double* turns;
   double m;
   int Hkv, Hq, D, rot, inter, pos32, items, hgroups;
+  int qheads;                                  // query heads of a workgroup
 };
 
 __device__ __forceinline__ double position_of(const AppendArgs& a, int64_t t, int64_t own) {
@@ -134,6 +137,31 @@ __device__ __forceinline__ void finite_max(float x, float& amax, bool& bad) {
   else bad = true;
 }
 
+// Two results of each wave joined over the waves that share a head (by all threads of the workgroup).
+template <class T, class F>
+__device__ __forceinline__ void over_waves(T& x, T& y, F join) {
+  __shared__ T all[4][2];
+  __syncthreads();
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    all[w][0] = x;
+    all[w][1] = y;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x = join(x, all[i][0]);
+    y = join(y, all[i][1]);
+  }
+}
+__device__ __forceinline__ void finish_maxima(float& mk, float& mv, bool& bk, bool& bv) {
+  over_waves(mk, mv, [](float x, float y) { return fmaxf(x, y); });
+  int ik = bk, iv = bv;
+  over_waves(ik, iv, [](int x, int y) { return x | y; });
+  bk = ik != 0;
+  bv = iv != 0;
+}
+
 // A unit of a key and of its value into the slot's row.
 template <int DT, int CT, int UP>
 __device__ __forceinline__ void put(uint8_t* row, RopeUnit rk, RopeUnit rv, int D, const float* x, const float* y,
@@ -152,10 +180,11 @@ __device__ __forceinline__ void put(uint8_t* row, RopeUnit rk, RopeUnit rv, int 
 
 // A page's largest magnitudes, scales and old codes: from the largest finite magnitudes of the new keys and values (of the
 // whole wave) and whether any is not finite, the scales to write with.  ok, ov: the page's scales before.
+// `first`, `step`: the caller's share of the old codes.
 template <int CT, int UP>
-__device__ __forceinline__ void settle(const AppendArgs& a, uint8_t* base, float* sc, int s0, int n, float mk, float mv, bool bk,
+__device__ __forceinline__ void settle(const AppendArgs& a, int first, int step, uint8_t* base, float* sc, int s0, int n, float mk, float mv, bool bk,
                                        bool bv, float ok, float ov, float& sk, float& sv) {
-  const int lane = threadIdx.x & 63, N = a.st.N, D = a.D;
+  const int N = a.st.N, D = a.D;
   sk = scale_for<CT>(mk);
   sv = scale_for<CT>(mv);
   if (CT == SDC_CACHE_I8 && bk) sk = __builtin_nanf("");
@@ -168,7 +197,7 @@ __device__ __forceinline__ void settle(const AppendArgs& a, uint8_t* base, float
     if (gk || gv) {
       constexpr int C = UP == 8 ? 8 : 1;
       const int nc = D / C;
-      for (int i = lane; i < (N - n) * nc; i += 64) {
+      for (int i = first; i < (N - n) * nc; i += step) {
         int s = i / nc;
         const int c = (i - s * nc) * C;
         if (s >= s0) s += n;
@@ -178,13 +207,14 @@ __device__ __forceinline__ void settle(const AppendArgs& a, uint8_t* base, float
       }
     }
   }
-  if (lane == 0) {
+  if (first == 0) {
     sc[0] = sk;
     sc[1] = sv;
   }
 }
 
-template <int DT, int CT, int UP>
+// SHARE waves of the workgroup (1, or all 4) on one head.
+template <int DT, int CT, int UP, int SHARE>
 __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int hg, float2* tab) {
   typedef typename RopeElem<DT>::T E;
   const PagedStep& st = a.st;
@@ -202,8 +232,9 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   const int32_t page = st.bt[r * st.sbt + w];
   const int n = (int)(hi - lo), s0 = (int)(lo - w * N);
   const int64_t t0 = rq.q1 - rq.len + lo;
-  const int h = hg * 4 + (tid >> 6);
+  const int h = SHARE == 4 ? hg : hg * 4 + (tid >> 6);
   const bool live = h < a.Hkv;
+  const int mine = SHARE == 4 ? tid : lane, step = 64 * SHARE;          // the wave's part of the head's units
   const E* kp = (const E*)a.k + (live ? h : 0) * a.skh;
   const E* vp = (const E*)a.v + (live ? h : 0) * a.svh;
   const int units = n * nu;
@@ -211,13 +242,13 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   // Up to HELD units a lane stay in registers, all loads of keys and values on their way at once (a token of 64 sequences each:
   // 6.6 us, 12 with the two passes below, which larger pages take).
   constexpr int HELD = 2;
-  if (units <= 64 * HELD && n * P <= TAB) {
+  if (units <= step * HELD && n * P <= TAB) {
     float x[HELD][2 * UP], y[HELD][2 * UP];
     RopeUnit ru[HELD], rv[HELD];
     int tok[HELD];
 #pragma unroll
     for (int j = 0; j < HELD; ++j) {
-      const int i = lane + 64 * j;
+      const int i = mine + step * j;
       const bool on = live && i < units;
       tok[j] = on ? i / nu : -1;
       const int t = on ? tok[j] : 0, u = on ? i - t * nu : 0;
@@ -244,7 +275,6 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
       tab[i] = sdc_turn(position_of(a, t0 + t, lo + t), i < 256 || 256 % P == 0 ? turn : a.turns[i - t * P], a.m);
     }
     __syncthreads();
-    if (!live) return;
     // the largest magnitudes as bits, of which those of infinities and NaN are the largest
     uint32_t uk = 0, uv = 0;
 #pragma unroll
@@ -261,6 +291,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
     if constexpr (CT != SDC_CACHE_16) {
       uk = wave_max_u32_dpp(uk);
       uv = wave_max_u32_dpp(uv);
+      if constexpr (SHARE > 1) over_waves(uk, uv, [](uint32_t x, uint32_t y) { return max(x, y); });
       float mk = __uint_as_float(uk), mv = __uint_as_float(uv);
       bool bk = false, bv = false;
       plain = max(uk, uv) < 0x7F800000u;
@@ -275,8 +306,12 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
           }
         mk = wave_max_f32_dpp(mk);
         mv = wave_max_f32_dpp(mv);
+        bk = __any(bk);
+        bv = __any(bv);
+        if constexpr (SHARE > 1) finish_maxima(mk, mv, bk, bv);
       }
-      settle<CT, UP>(a, base, sc, s0, n, mk, mv, __any(bk), __any(bv), ok, ov, sk, sv);
+      if (!live) return;
+      settle<CT, UP>(a, mine, step, base, sc, s0, n, mk, mv, bk, bv, ok, ov, sk, sv);
     }
     const Divide dk(sk), dv(sv);
     plain = plain && dk.pow2 && dv.pow2;
@@ -317,7 +352,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
     bool bk = false, bv = false;
     for (int first = 0; first < n; first += rows) {
       const int m = angles(first);
-      for (int i = lane; live && i < m * nu; i += 64) {
+      for (int i = mine; live && i < m * nu; i += step) {
         const int t = i / nu, u = i - t * nu;
         float x[2 * UP], y[2 * UP];
         key(first, t, u, x);
@@ -329,16 +364,21 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
         }
       }
     }
+    mk = wave_max_f32_dpp(mk);
+    mv = wave_max_f32_dpp(mv);
+    bk = __any(bk);
+    bv = __any(bv);
+    if constexpr (SHARE > 1) finish_maxima(mk, mv, bk, bv);
     if (live) {
       float* sc = a.scales + (int64_t)page * a.sb + h * a.sh;
       const float ok = s0 > 0 ? sc[0] : 0.f, ov = s0 > 0 ? sc[1] : 0.f;
-      settle<CT, UP>(a, base, sc, s0, n, wave_max_f32_dpp(mk), wave_max_f32_dpp(mv), __any(bk), __any(bv), ok, ov, sk, sv);
+      settle<CT, UP>(a, mine, step, base, sc, s0, n, mk, mv, bk, bv, ok, ov, sk, sv);
     }
   }
   const Divide dk(sk), dv(sv);
   for (int first = 0; first < n; first += rows) {
     const int m = (CT != SDC_CACHE_16 && rows >= n) ? n : angles(first);
-    for (int i = lane; live && i < m * nu; i += 64) {
+    for (int i = mine; live && i < m * nu; i += step) {
       const int t = i / nu, u = i - t * nu;
       float x[2 * UP], y[2 * UP];
       const RopeUnit rk = key(first, t, u, x), rv = value(first, t, u, y);
@@ -350,14 +390,14 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
 // The queries of QTOK tokens, rotated; those past the last request are written as zeros.  A thread's first unit is on its
 // way while the tokens' requests are found.
 template <int DT, int UP>
-__device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t block, float2* tab) {
+__device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t block, int h0, float2* tab) {
   typedef typename RopeElem<DT>::T E;
   constexpr int HELD = 1;
   const int tid = threadIdx.x, P = a.rot / 2, nu = sdc_units(a.D, UP);
   const int TB = P ? min(QTOK, TAB / P) : QTOK;
   __shared__ int64_t own[QTOK];                                         // the tokens' positions in their requests
   for (int64_t t0 = block * QTOK, te = min(t0 + QTOK, a.st.T); t0 < te; t0 += TB) {
-    const int nt = (int)min((int64_t)TB, te - t0), all = nt * a.Hq * nu;
+    const int nt = (int)min((int64_t)TB, te - t0), nh = min(a.qheads, a.Hq - h0), all = nt * nh * nu;
     struct Unit {
       int t, h;
       RopeUnit ru;
@@ -365,8 +405,8 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t bloc
     };
     auto load = [&](int i, Unit& u) {
       const int th = i / nu;
-      u.t = th / a.Hq;
-      u.h = th - u.t * a.Hq;
+      u.t = th / nh;
+      u.h = h0 + th - u.t * nh;
       u.ru = sdc_unit<UP>(i - th * nu, a.rot, a.inter);
       sdc_load_unit<DT, UP>((const E*)a.q + (t0 + u.t) * a.sqt + u.h * a.sqh, a.sqd, u.ru, a.D, u.x);
     };
@@ -408,19 +448,29 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t bloc
   }
 }
 
-template <int DT, int CT, int UP>
+template <int DT, int CT, int UP, int SHARE>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   __shared__ float2 tab[TAB];
   const int64_t b = blockIdx.x, pages = (int64_t)a.items * a.hgroups;
-  if (b < pages) append_page<DT, CT, UP>(a, (int)(b / a.hgroups), (int)(b % a.hgroups), tab);
-  else rotate_queries<DT, UP>(a, b - pages, tab);
+  if (b < pages) append_page<DT, CT, UP, SHARE>(a, (int)(b / a.hgroups), (int)(b % a.hgroups), tab);
+  else {
+    const int groups = (a.Hq + a.qheads - 1) / a.qheads;
+    rotate_queries<DT, UP>(a, (b - pages) / groups, (int)((b - pages) % groups) * a.qheads, tab);
+  }
 }
 template <int DT, int CT, int UP>
-int launch(const AppendArgs& a, hipStream_t stream) {
-  const int64_t blocks = (int64_t)a.items * a.hgroups + (a.q ? sdc_cdiv(a.st.T, QTOK) : 0);
+int launch(AppendArgs a, hipStream_t stream) {
+  // four waves share a head where a page holds more units than one keeps in registers (64 slots of 128: 200 tokens in
+  // four chunks 24 us, 33 with a wave a head); a workgroup takes up to 1024 units of queries
+  const int nu = sdc_units(a.D, UP);
+  const bool share = a.st.N * nu > 128;
+  a.hgroups = share ? a.Hkv : (int)sdc_cdiv(a.Hkv, 4);
+  a.qheads = std::min(std::max(a.Hq, 1), std::max(1, 1024 / (QTOK * nu)));
+  const int64_t blocks = (int64_t)a.items * a.hgroups + (a.q ? sdc_cdiv(a.st.T, QTOK) * sdc_cdiv(a.Hq, a.qheads) : 0);
   if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
   SdcProf prof("kv_append", stream);
-  hipLaunchKernelGGL((kv_append_kernel<DT, CT, UP>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  if (share) hipLaunchKernelGGL((kv_append_kernel<DT, CT, UP, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((kv_append_kernel<DT, CT, UP, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
   SDC_LAUNCH_CHECK();
   return SDC_OK;
 }
@@ -482,6 +532,5 @@ extern "C" int sdc_kv_append(int dtype, int cache, const void* key, int64_t skt,
   const int64_t items = T / N + 2 * R;
   if (items > 0x3FFFFFFF) return SDC_EUNSUPPORTED;
   a.items = (int)items;
-  a.hgroups = (int)sdc_cdiv(Hkv, 4);
   return dtype == SDC_BF16 ? pick_cache<SDC_BF16>(cache, a, stream) : pick_cache<SDC_FP16>(cache, a, stream);
 }

@@ -637,7 +637,9 @@ __device__ __forceinline__ float over_halves_sum(float v) {
 template <int CT, int DP, int PN>
 __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_attend_tiles(AttendArgs a, Split sp) {
   constexpr int KT = DP > 128 ? 32 : 64, KB = KT / 32;                  // keys of a tile, blocks of 32
-  constexpr int NS = DP / 16, ND = DP / 32;                             // depth steps of a score, row blocks of the output
+  // depth steps of a score; the values' rows, by which of a dword's four codes they are, and blocks of 32 of them (a head of
+  // 96 in quarters of 32, 8 of them unused: a lane then has adjacent outputs)
+  constexpr int NS = DP / 16, VR = DP == 96 ? 32 : DP / 4, ND = 4 * VR / 32;
   constexpr int KP = 2 * DP + 16, VP = 2 * KT + 16;                     // row pitches in bytes
   constexpr int NW = tall_waves(DP), TALL = 32 * NW, HT = 32 * NW;      // half of the threads load keys, half values
   // reads of a key and of a thread, 16 codes each; columns of 4 codes of a value, units (8 keys x 4 codes) of a thread
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   constexpr float BIAS = 13.f;
   struct Stage {
     uint8_t k[KT * KP];
-    uint8_t v[DP * VP];
+    uint8_t v[4 * VR * VP];
     float4 sc[KT];                             // of each key, as of its page
   };
   __shared__ Stage st[2];
@@ -690,26 +692,10 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   const int64_t a0 = t.c0 + (int64_t)s * t.C, a1 = min(t.khi, a0 + t.C);
   const int64_t fp = (uint32_t)a0 / (uint32_t)N;
   const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
-  // The part's pages and their scales.  A page outside the cache is page 0 with scales of NaN.  Value scales that have no
-  // logarithm (0, infinity, NaN) become factors on the widened values, and so do signs; a key scale of NaN makes the page's
-  // share of the sum and its values NaN.
-  bool flip = false, mul = false;
-  for (int i = tid; i < np; i += 2 * HT) {
-    const int32_t p = a.st.bt[t.r * a.st.sbt + fp + i];
-    const bool in = p >= 0 && p < a.st.NB;
-    const float* scp = a.scales + (in ? (int64_t)p : 0) * a.sb + t.hk * a.sh;
-    const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf(""), v = fabsf(vs);
-    const bool log = v > 0.f && v < __builtin_inff(), key = ks == ks;
-    ps[i] = {key ? fabsf(ks) : 0.f, log ? log2f(v) : 0.f, !key ? ks : log ? fminf(1.f / v, 0x1p126f) : 1.f,
-             !key ? ks : !log ? vs : vs < 0.f ? -1.f : 1.f};
-    pg[i] = (in ? p : 0) | (ks < 0.f ? (int32_t)0x80000000 : 0);        // the sign of ks, which the keys take
-    flip |= ks < 0.f;
-    mul |= !log || vs < 0.f || !key;
-  }
-
   // the queries: fragments of the lane's row, in fp16 after a power of two
   f16x8 qf[NS];
   float rf;
+  bool flip = false, mul = false;
   int64_t prow;                                // the lane's position
   {
     const Row r = row_of();
@@ -731,6 +717,21 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       }
     }
     int e = 0;
+    // The part's pages and their scales.  A page outside the cache is page 0 with scales of NaN.  Value scales that have no
+    // logarithm (0, infinity, NaN) become factors on the widened values, and so do signs; a key scale of NaN makes the page's
+    // share of the sum and its values NaN.
+    for (int i = tid; i < np; i += 2 * HT) {
+      const int32_t p = a.st.bt[t.r * a.st.sbt + fp + i];
+      const bool in = p >= 0 && p < a.st.NB;
+      const float* scp = a.scales + (in ? (int64_t)p : 0) * a.sb + t.hk * a.sh;
+      const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf(""), v = fabsf(vs);
+      const bool log = v > 0.f && v < __builtin_inff(), key = ks == ks;
+      ps[i] = {key ? fabsf(ks) : 0.f, log ? log2f(v) : 0.f, !key ? ks : log ? fminf(1.f / v, 0x1p126f) : 1.f,
+               !key ? ks : !log ? vs : vs < 0.f ? -1.f : 1.f};
+      pg[i] = (in ? p : 0) | (ks < 0.f ? (int32_t)0x80000000 : 0);        // the sign of ks, which the keys take
+      flip |= ks < 0.f;
+      mul |= !log || vs < 0.f || !key;
+    }
     auto narrow = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
 #pragma unroll
@@ -911,7 +912,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f16x8*>(d.v + lds + e * (DP / 4) * VP + 16 * (HT / VC) * u) = v[e];
+        *reinterpret_cast<f16x8*>(d.v + lds + e * VR * VP + 16 * (HT / VC) * u) = v[e];
     }
     if (half < KT) {
       int slot;
@@ -1021,18 +1022,21 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   // In the step of tile t the waves take the values of t and the keys of t + 1.  At its start the values of t + 1 and the keys of
   // t + 2, loaded during the step before, are put where the values of t - 1 and the keys of t were.
   Next n;
-  find(0);
-  load(0, n);
-  store(0, n, st[0]);
-  if (KT < nk) {
-    find(KT);
-    load(KT, n);
-    if (!vals) {
-      store(KT, n, st[1]);
-      if (2 * KT < nk) {
-        find(2 * KT);
-        load(2 * KT, n);
-      }
+  {
+    Next first;
+    find(0);
+    load(0, first);
+    if (KT < nk) {
+      find(KT);
+      load(KT, n);
+    }
+    store(0, first, st[0]);
+  }
+  if (!vals && KT < nk) {
+    store(KT, n, st[1]);
+    if (2 * KT < nk) {
+      find(2 * KT);
+      load(2 * KT, n);
     }
   }
   const int ahead = vals ? KT : 2 * KT;
@@ -1054,30 +1058,22 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     if (k + KT < nk) step(k + KT, st[1], st[0], xb, xa);
   }
 
-  // o[q][i] of a lane is element 4 (p % (DP / 4)) + p / (DP / 4), p = 32 q + 8 (i / 4) + 4 h + i % 4: the values' rows lie in that
-  // order, which gives a lane four adjacent elements (not of 96, whose quarters are no blocks)
+  // o[q][i] of a lane is element 4 (p % VR) + p / VR, p = 32 q + 8 (i / 4) + 4 h + i % 4: the values' rows lie in that order
   auto element = [&](int q, int i) {
     const int p = 32 * q + 8 * (i / 4) + 4 * h + i % 4;
-    return 4 * (p % (DP / 4)) + p / (DP / 4);
+    return 4 * (p % VR) + p / VR;
   };
-  auto each = [&](auto use4, auto use1) {
-    if constexpr (DP != 96) {
-      constexpr int B = DP / 128 > 0 ? DP / 128 : 1, E = DP == 64 ? 8 : 16;    // blocks and registers of a quarter's rows
+  auto each = [&](auto use) {                  // four adjacent elements at a time
+    constexpr int B = VR > 32 ? VR / 32 : 1, E = VR < 32 ? 8 : 16;      // blocks and registers of a quarter's rows
 #pragma unroll
-      for (int b = 0; b < B; ++b)
+    for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          f32x4 x;
+      for (int i = 0; i < E; ++i) {
+        f32x4 x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = DP == 64 ? o[e / 2][i + 8 * (e % 2)] : o[b + B * e][i];
-          use4(element(b, i), x);
-        }
-    } else {
-#pragma unroll
-      for (int q = 0; q < ND; ++q)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) use1(element(q, i), o[q][i]);
-    }
+        for (int e = 0; e < 4; ++e) x[e] = VR < 32 ? o[e / 2][i + 8 * (e % 2)] : o[b + B * e][i];
+        if (element(b, i) < D) use(element(b, i), x);
+      }
   };
   if (__syncthreads_or(bad)) {                 // values that were left out: NaN for the rows that see them
     for (int key = max(lo0, rlo); key < rhi; ++key) {
@@ -1105,9 +1101,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     const int64_t p = t.p0 + r.tok;
     const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
     const float f = any ? 1.f / l : 0.f;
-    each([&](int d, f32x4 x) {
-      if (d < D) write_four(a, r.token, r.head, d, x, f);
-    }, [&](int d, float x) { write_out(a, r.token, r.head, d, &x, 1, f); });
+    each([&](int d, f32x4 x) { write_four(a, r.token, r.head, d, x, f); });
     if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = any ? (m + log2f(l) - BIAS) * LN2 : NEG_INF;
   } else {
     float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + 2);
@@ -1115,11 +1109,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       rec[2 * r.row] = m;
       rec[2 * r.row + 1] = l * 0x1p-13f;
     }
-    each([&](int d, f32x4 x) {
-      if (d < D) *reinterpret_cast<f32x4*>(rec + 2 * TALL + r.row * D + d) = x * 0x1p-13f;
-    }, [&](int d, float x) {
-      if (d < D) rec[2 * TALL + r.row * D + d] = x * 0x1p-13f;
-    });
+    each([&](int d, f32x4 x) { *reinterpret_cast<f32x4*>(rec + 2 * TALL + r.row * D + d) = x * 0x1p-13f; });
   }
 }
 
@@ -1162,14 +1152,31 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split rows, 
   const float* ml = rec + 2 * row;
   const float* v = rec + 2 * sp.rows + row * D + d;
   float m = M0, l = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < t.nsp; ++s) m = fmaxf(m, ml[s * size]);
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = 0; s < t.nsp; ++s) {
-    const float f = __builtin_amdgcn_exp2f(ml[s * size] - m);
-    l = fmaf(f, ml[s * size + 1], l);
-    x += f * *reinterpret_cast<const f32x4*>(v + s * size);
+  constexpr int U = 4;                         // parts whose loads are on their way at once
+  for (int b = 0; b < t.nsp; b += U) {
+    float2 w[U];
+    f32x4 y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t at = min(b + i, t.nsp - 1) * size;
+      w[i] = *reinterpret_cast<const float2*>(ml + at);
+      y[i] = *reinterpret_cast<const f32x4*>(v + at);
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mn = fmaxf(mn, w[i].x);
+    const float f = __builtin_amdgcn_exp2f(m - mn);
+    l *= f;
+    x *= f;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (b + i < t.nsp) {
+        const float g = __builtin_amdgcn_exp2f(w[i].x - m);
+        l = fmaf(g, w[i].y, l);
+        x += g * y[i];
+      }
   }
   const int64_t p = t.p0 + tok;
   const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
