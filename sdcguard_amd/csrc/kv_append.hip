@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int TAB = 1024;                      // (cos, sin) pairs a workgroup holds
+constexpr int TAB = 1024, WIDE = 4096;         // (cos, sin) pairs a workgroup holds; of large pages
 constexpr int QTOK = 4;                        // tokens a workgroup of the queries' rotation takes
 
 struct AppendArgs {
@@ -217,6 +217,7 @@ __device__ __forceinline__ void settle(const AppendArgs& a, int first, int step,
 template <int DT, int CT, int UP, int SHARE>
 __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int hg, float2* tab) {
   typedef typename RopeElem<DT>::T E;
+  constexpr int HOLD = SHARE > 1 ? WIDE : TAB;
   const PagedStep& st = a.st;
   const int N = st.N, D = a.D, tid = threadIdx.x, lane = tid & 63;
   const int P = a.rot / 2, nu = sdc_units(D, UP);
@@ -242,7 +243,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   // Up to HELD units a lane stay in registers, all loads of keys and values on their way at once (a token of 64 sequences each:
   // 6.6 us, 12 with the two passes below, which larger pages take).
   constexpr int HELD = 2;
-  if (units <= step * HELD && n * P <= TAB) {
+  if (units <= step * HELD && n * P <= HOLD) {
     float x[HELD][2 * UP], y[HELD][2 * UP];
     RopeUnit ru[HELD], rv[HELD];
     int tok[HELD];
@@ -322,7 +323,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   }
 
   if (page < 0 || page >= st.NB) return;
-  const int rows = P ? min(n, TAB / P) : n;                             // tokens whose angles are held at once
+  const int rows = P ? min(n, HOLD / P) : n;                             // tokens whose angles are held at once
   uint8_t* base = a.kv + (int64_t)page * a.cb + (live ? h : 0) * a.ch;
   auto angles = [&](int first) {                                        // by the whole workgroup
     const int m = min(rows, n - first);
@@ -450,7 +451,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t bloc
 
 template <int DT, int CT, int UP, int SHARE>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
-  __shared__ float2 tab[TAB];
+  __shared__ float2 tab[SHARE > 1 ? WIDE : TAB];
   const int64_t b = blockIdx.x, pages = (int64_t)a.items * a.hgroups;
   if (b < pages) append_page<DT, CT, UP, SHARE>(a, (int)(b / a.hgroups), (int)(b % a.hgroups), tab);
   else {
