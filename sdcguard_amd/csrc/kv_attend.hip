@@ -1189,6 +1189,7 @@ struct Plan {
   Split rows, tiles;
   bool tall;                                   // kv_attend_tiles takes the requests of more than tiles.few tokens
 };
+constexpr int64_t CROSS = 640000000;           // small tiles x their keys x head size from which large ones are faster
 constexpr int FEW = 2;                         // kv_attend_rows takes requests of up to so many of its tiles, beside chunks
 Split split_of(int rows, int64_t G, int64_t N) {
   Split sp{};
@@ -1219,8 +1220,12 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
   // four of 100-131k 179 us, 32 of 1000-4000 with their append 44 us (three rounds: 34.5, 184 and 45).  Parts of fewer than 512
   // keys cost more to join than they save.  (Workgroups of eight waves, one a CU: 41, 182 and 42.)
   constexpr int64_t resident = 512;
-  // more tokens than requests: some have a chunk
-  p.tall = T > R && T > FEW * p.rows.TB;
+  // More tokens than requests: some have a chunk.  The tiles of 16 rows read every key anew, those of 256 cost two more
+  // launches and fill the chip later: chunks behind 4096 keys, 32 heads, 127 / 505 / 1009 / 2017 tokens in small and in large
+  // tiles, heads of 128: 52 and 57 / 97 and 107 / 172 and 141 / 290 and 188 us, heads of 64: 33 and 42 / 58 and 76 / 96 and
+  // 99 / 157 and 132 us.
+  const int64_t small = (T / p.rows.TB + R) * Hkv * p.rows.NHB;
+  p.tall = T > R && T > FEW * p.rows.TB && small * keys(p.rows) >= CROSS / D;
   if (p.tall) {
     p.tiles.few = p.rows.TB * FEW;
     p.rows.slots = FEW;
