@@ -349,6 +349,9 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
 
   float sk = 1.f, sv = 1.f;
   if constexpr (CT != SDC_CACHE_16) {
+    // (read before the barriers behind which one of the head's waves writes them)
+    float* sc = a.scales + (int64_t)page * a.sb + (live ? h : 0) * a.sh;
+    const float ok = s0 > 0 ? sc[0] : 0.f, ov = s0 > 0 ? sc[1] : 0.f;
     float mk = 0.f, mv = 0.f;
     bool bk = false, bv = false;
     for (int first = 0; first < n; first += rows) {
@@ -371,8 +374,6 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
     bv = __any(bv);
     if constexpr (SHARE > 1) finish_maxima(mk, mv, bk, bv);
     if (live) {
-      float* sc = a.scales + (int64_t)page * a.sb + h * a.sh;
-      const float ok = s0 > 0 ? sc[0] : 0.f, ov = s0 > 0 ? sc[1] : 0.f;
       settle<CT, UP>(a, mine, step, base, sc, s0, n, mk, mv, bk, bv, ok, ov, sk, sv);
     }
   }

@@ -144,3 +144,15 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("N,D", [(64, 128), (256, 128), (200, 96), (256, 40)])
+def test_append_of_chunks_into_large_pages(N, D, kind):
+    """Pages that several waves share, in one pass and in two, new and grown."""
+    c = make(((300, 300), (500, 200), (257, 1)), D=D, Hq=2, Hkv=3, N=N, kind=kind, seed=N + D, garbage=False)
+    append_checked(c, _turns(D))
+    c["k"].mul_(64.0)                                  # the same step again, its scales grown over the older codes
+    c["lens"].add_(1)
+    c["bt"][c["bt"] < 0] = c["kv"].shape[0] - 1
+    append_checked(c, _turns(D))
