@@ -1326,7 +1326,8 @@ extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, i
     return SDC_EINVAL;
   if (T == 0) return SDC_OK;
   if (!q || !o || !kv || !scales || !qsl || !seq_lens || !bt) return SDC_EINVAL;
-  if (T > 0x3FFFFFFF || R > 0x0FFFFFFF || Hq > 65536 || W * N > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
+  if (T > 0x3FFFFFFF || R > 0x0FFFFFFF || Hq > 65536 || W * N > 0x7FFFFFFF || max_len > 0x3FFFFFFF)
+    return SDC_EUNSUPPORTED;                    // (numbers of keys are added up in 32 bits)
   AttendArgs a{};
   a.st = PagedStep{qsl, seq_lens, bt, sbt, W, NB, T, (int)R, (int)N};
   a.q = (const uint16_t*)q; a.o = (uint16_t*)o; a.lse = lse;
