@@ -142,7 +142,7 @@ def bound():
                                           "`python -m sdcguard_amd.csrc.build`") from e
                 _bind.bind(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in
                              ("sdc_rope", "sdc_kv_append", "sdc_kv_attend_workspace", "sdc_kv_attend")),
-                           _raw_stream_at, check, HipLibraryError)
+                           check, HipLibraryError)
                 _bound[0] = _bind
     return _bound[0]
 
@@ -166,13 +166,6 @@ def _raw_stream(device: torch.device) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index
     return _current_raw_stream(torch.cuda.current_device() if index is None else index)
-
-
-def _stream_at(index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
-
-
-_raw_stream_at = _current_raw_stream or _stream_at
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -6,6 +6,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -29,7 +30,6 @@ struct Entry {
   decltype(&sdc_kv_attend) attend;
 };
 Entry g_entry;
-PyObject* g_stream = nullptr;                  // torch's query of a device's current raw stream
 PyObject* g_check = nullptr;                   // _lib.check: raises for a status
 PyObject* g_error = nullptr;                   // _lib.HipLibraryError
 
@@ -72,17 +72,8 @@ int half_code(const Tensor& t) {
   refuse(g_error, std::string("unsupported dtype ") + c10::toString(t.scalar_type()));
 }
 
-hipStream_t stream_of(const Tensor& t) {
-  PyObject* index = PyLong_FromLong(t.device().index());
-  if (!index) throw Raised{};
-  PyObject* r = PyObject_CallOneArg(g_stream, index);
-  Py_DECREF(index);
-  if (!r) throw Raised{};
-  void* s = PyLong_AsVoidPtr(r);
-  Py_DECREF(r);
-  if (!s && PyErr_Occurred()) throw Raised{};
-  return (hipStream_t)s;
-}
+// (torch's own state, asked without Python: a gradient's thread would have to wait for the interpreter's lock)
+hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 void check(int rc, const char* what) {
   if (rc == 0) return;
@@ -156,8 +147,7 @@ struct Rotation : torch::autograd::Function<Rotation> {
     ctx->saved_data["inverse"] = inverse;
     const Tensor y = like(x);
     const c10::DeviceGuard guard(x.device());
-    const hipStream_t s = locked([&] { return stream_of(x); });
-    const int rc = launch_rotation(x, y, pos, turns, How{interleaved, inverse, mscale}, s);
+    const int rc = launch_rotation(x, y, pos, turns, How{interleaved, inverse, mscale}, stream_of(x));
     if (rc != 0) locked([&] { check(rc, "sdc_rope"); });
     return y;
   }
@@ -384,10 +374,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of sdc_rope, sdc_kv_append, sdc_kv_attend_workspace, sdc_kv_attend; the stream query; check; HipLibraryError)
+// bind(addresses of sdc_rope, sdc_kv_append, sdc_kv_attend_workspace, sdc_kv_attend; check; HipLibraryError)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "7 arguments expected");
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "6 arguments expected");
     return nullptr;
   }
   void* p[4];
@@ -400,8 +390,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   g_entry = Entry{(decltype(&sdc_rope))p[0], (decltype(&sdc_kv_append))p[1], (decltype(&sdc_kv_attend_workspace))p[2],
                   (decltype(&sdc_kv_attend))p[3]};
-  PyObject** keep[3] = {&g_stream, &g_check, &g_error};
-  for (int i = 0; i < 3; ++i) {
+  PyObject** keep[2] = {&g_check, &g_error};
+  for (int i = 0; i < 2; ++i) {
     Py_INCREF(a[4 + i]);
     Py_XSETREF(*keep[i], a[4 + i]);
   }
