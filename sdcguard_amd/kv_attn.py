@@ -61,7 +61,8 @@ def kv_attend(q: torch.Tensor, kv: torch.Tensor, scales: torch.Tensor, qsl: torc
     exp(scale q . k).
 
     scale: head size ** -0.5 unless given.  window > 0: a query sees the last `window` keys, its own included.
-    max_seq_len: a bound on seq_lens that the host knows (default: what the table holds); keys past it are not read.
+    max_seq_len: a bound on seq_lens that the host knows (default: what the table holds); keys past it are not read, and
+    the call plans its workspace and kernels for it, so a bound near the lengths is faster.
     A query that sees no key, and the padding's, get zeros and -inf.  A page of a query's keys that lies outside the
     cache makes its output NaN."""
     return _lib.bound().attend(q, kv, scales, qsl, seq_lens, bt, scale, window, max_seq_len, out, return_lse)
