@@ -1231,10 +1231,16 @@ void cut(Split& sp, int64_t busy, int64_t want, int64_t least, int64_t keys, int
   // (a tile's keys over S parts, rounded up to 128, must stay within `most`)
   sp.S = (int)std::max<int64_t>({1, s, sdc_cdiv(keys, most)});
 }
+// The keys a query sees at most: without a window, or with one so wide that sums with it could pass 64 bits, more than any
+// length.
+int64_t seen(int64_t window) {
+  constexpr int64_t all = (int64_t)1 << 40;
+  return window > 0 ? std::min(window, all) : all;
+}
 Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, int64_t max_len, int64_t window) {
   Plan p{};
   // keys a tile's rows can see together
-  auto keys = [&](const Split& sp) { return window > 0 ? std::min(max_len, window + sp.TB) : max_len; };
+  auto keys = [&](const Split& sp) { return std::min(max_len, seen(window) + sp.TB); };
   p.rows = split_of(ROWS, G, N);
   p.tiles = split_of(32 * tall_waves(D), G, N);
   // One round of the workgroups that a lane's registers leave room for, two a CU: 64 sequences of 512-2048 tokens 34.5 us,
@@ -1356,7 +1362,7 @@ extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, i
   a.scales = scales; a.sb = sb; a.sh = sh;
   a.scale = scale * LOG2E;
   a.maxlen = max_len;
-  a.window = window > 0 ? window : (int64_t)1 << 40;
+  a.window = seen(window);
   a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.D = (int)D; a.fp16 = dtype == SDC_FP16;
   // the tiled kernels read 16 codes at a time, and divide by N by a product (exact up to this many slots)
   if (D % 16 == 0 && N <= 4096 && cn >= 0 && cn < (1 << 19) && ((uintptr_t)kv | (uintptr_t)(cb | ch | cn)) % 16 == 0) {

@@ -97,3 +97,12 @@ def test_frequencies_of_scaled_rotations():
         assert t[0] == plain[0] and math.isclose(t[-1].item(), plain[-1].item() / 8, rel_tol=1e-12)
         assert ((t <= plain) & (t >= plain / 8 * (1 - 1e-12))).all() and (t[:-1] > t[1:]).all()
         assert m == (1.0 + 0.1 * math.log(8.0) if kind == "ramp" else 1.0)
+
+
+@pytest.mark.parametrize("window", [(1 << 63) - 1, (1 << 63) - 16, 1 << 62, 1 << 40, 1 << 31])
+def test_a_window_wider_than_any_length_is_none(window):
+    """The parts that a call's keys are cut into, by the workspace that they need."""
+    need = _lib.lib().sdc_kv_attend_workspace
+    for T, R, N, most in ((1, 1, 16, 200000), (1, 1, 1, 5000), (64, 64, 16, 131072), (4096, 2, 16, 131072), (3, 0, 8, 70000)):
+        assert need(T, R, 32, 8, 128, N, most, window) == need(T, R, 32, 8, 128, N, most, 0)
+    assert need(1, 1, 32, 8, 128, 16, 200000, window) > 0
