@@ -40,7 +40,7 @@ def smallest_scale(amax, kind):
         e -= 1
     while 2.0 ** e * TOP[kind] < amax:
         e += 1
-    return 2.0 ** min(max(e, -126), 120)
+    return 2.0 ** max(e, -126)
 
 
 def half_step(x, scale, kind):

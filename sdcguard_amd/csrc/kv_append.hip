@@ -45,7 +45,8 @@ __device__ __forceinline__ double position_of(const AppendArgs& a, int64_t t, in
   return a.pos32 ? (double)((const int32_t*)a.pos)[t] : (double)((const int64_t*)a.pos)[t];
 }
 
-// the smallest power of two whose product with the largest code holds amax
+// the smallest power of two whose product with the largest code holds amax (at most 2^120 for e4m3 and 2^122 for int8, of
+// values next to 2^128: reciprocals are normal numbers), 2^-126 at least
 template <int CT>
 __device__ __forceinline__ float scale_for(float amax) {
   if (amax == 0.f) return 0x1p-126f;
@@ -53,7 +54,7 @@ __device__ __forceinline__ float scale_for(float amax) {
   const float f = frexpf(amax, &e);                                     // f in [0.5, 1)
   constexpr float top = CT == SDC_CACHE_E4M3 ? 0.875f : 127.f / 128.f;  // 448 / 2^9, 127 / 2^7
   e += (f > top) - (CT == SDC_CACHE_E4M3 ? 9 : 7);
-  return ldexpf(1.f, min(max(e, -126), 120));
+  return ldexpf(1.f, max(e, -126));
 }
 
 // x / S: a power of two's reciprocal is exact (S may be another quantizer's, of any value)

@@ -66,3 +66,11 @@ def test_attention_is_a_softmax_per_row():
     assert np.allclose(o[3, 0], kv[2, 0, 0, D:]) and (mass >= np.abs(o) - 1e-12).all()
     o, lse, _, _ = paged.attend(q, kv, [0, 4], [2], bt, N, 1.0)                     # two rows without a position
     assert not o[:2].any() and np.isneginf(lse[:2]).all() and o[2:].any()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_scales_hold_the_largest_values_of_32_bits(kind):
+    for amax in (2.0 ** 127, 127.0 * 2.0 ** 120, 127.5 * 2.0 ** 120, 2e38, 255.0 * 2.0 ** 120, 2.0 ** 128 * (1 - 2.0 ** -24)):
+        s = paged.smallest_scale(amax, kind)
+        assert s * paged.TOP[kind] >= amax > s / 2 * paged.TOP[kind]
+        assert s <= 2.0 ** (120 if kind == "e4m3" else 122)
