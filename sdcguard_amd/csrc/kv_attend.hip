@@ -6,7 +6,8 @@
 //
 // kv_attend_rows: tiles of 16 query rows, for decode steps and small chunks (HBM bound, or by latency).  kv_attend_tiles:
 // tiles of 256 query rows, for chunks of a prompt (bound by the matrix cores and the softmax between them).  kv_attend_any:
-// any head size and alignment.  A part of a tile's keys is one workgroup's; kv_attend_join joins the parts in their order.
+// any head size and alignment, a row a wave; kv_attend_rows leaves a part whose value scales are far from 1 to the same (plain_row).
+// A part of a tile's keys is one workgroup's; kv_attend_join joins the parts in their order.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,7 +37,8 @@ struct AttendArgs {
 // The work of a tiled kernel: tiles of TB query tokens x GB heads of one kv head (at most `rows` query rows), whose keys
 // are cut into at most S parts, one part a workgroup.  A call with chunks runs both kernels: requests of up to `few`
 // tokens go to kv_attend_rows, the others, and the padding, to kv_attend_tiles.
-// part: (tile, part) records of `rows` (maximum, sum) pairs and rows x D sums.
+// part: (tile, part) records: `rows` heads (the exponent of the row's sums of values, that of its sum of probabilities, which is
+// the maximum, and that sum, 0), then rows x D sums.
 struct Split {
   int64_t tiles;
   int TB, GB, NHB, S, rows;
@@ -55,30 +57,33 @@ __device__ __forceinline__ float value_of(uint32_t c) {
 
 constexpr int ANY_D = 256;                     // largest head size
 
-template <int DT, int CT>
-__global__ __launch_bounds__(256) void kv_attend_any(AttendArgs a) {
-  __shared__ float qs[4][ANY_D];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t id = (int64_t)blockIdx.x * 4 + w;
-  const bool live = id < a.st.T * a.Hq;
-  const int64_t t = live ? id / a.Hq : 0;
-  const int h = live ? (int)(id - t * a.Hq) : 0, hk = h / a.G;
-  const int D = a.D;
-  for (int d = lane; d < D; d += 64) qs[w][d] = half_to_f32<DT>(a.q[t * a.sqt + h * a.sqh + d * a.sqd]);
+// A value scale's exponent field: v < 2^(field - 126).  0 of zero, infinity and NaN.
+__device__ __forceinline__ uint32_t scale_field(float v) {
+  const uint32_t e = (__float_as_uint(v) >> 23) & 0xFFu;
+  return e == 0xFFu ? 0u : max(e, (uint32_t)(v != 0.f));
+}
+
+// A query into `row` (of the wave).
+__device__ __forceinline__ void plain_query(const AttendArgs& a, int64_t t, int h, float* row) {
+  const uint16_t* q = a.q + t * a.sqt + h * a.sqh;
+  sdc_wave_lds_fence();                        // (another row's may be read still)
+  for (int d = threadIdx.x & 63; d < a.D; d += 64)
+    row[d] = a.fp16 ? half_to_f32<SDC_FP16>(q[d * a.sqd]) : half_to_f32<SDC_BF16>(q[d * a.sqd]);
   sdc_wave_lds_fence();
-  if (!live) return;
-  Request rq;
-  int64_t first;
-  const int r = sdc_find_request(a.st, t, 1, 0, rq, first);
-  int64_t lo = 0, hi = 0;
-  if (r >= 0 && r < a.st.R) {
-    hi = min(t - rq.q1 + rq.len + 1, a.maxlen);
-    lo = max(t - rq.q1 + rq.len + 1 - a.window, (int64_t)0);
-  }
-  float m = NEG_INF, l = 0.f, o[ANY_D / 64] = {};
+}
+// One query row over keys lo .. hi of request r, by a wave, all in fp32: a lane has a key's score, then elements lane + 64 e of
+// the output, in units of 2^u where values would pass fp32 in their sum.
+struct PlainRow {
+  float m, l, o[ANY_D / 64];
+  int u;
+};
+template <int CT>
+__device__ __forceinline__ PlainRow plain_row(const AttendArgs& a, const float* q, int r, int hk, int64_t lo, int64_t hi) {
+  const int lane = threadIdx.x & 63, D = a.D;
+  PlainRow s{NEG_INF, 0.f, {}, 0};
   for (int64_t b = lo; b < hi; b += 64) {
     const int64_t j = b + lane;
-    float s = NEG_INF, vs = 0.f;
+    float x = NEG_INF, vs = 0.f;
     int64_t row = 0;
     if (j < hi) {
       const int64_t wp = j / a.st.N, page = a.st.bt[r * a.st.sbt + wp];
@@ -88,36 +93,68 @@ __global__ __launch_bounds__(256) void kv_attend_any(AttendArgs a) {
       const float ks = in ? sc[0] : __builtin_nanf("");
       vs = in ? sc[1] : __builtin_nanf("");
       float dot = 0.f;
-      for (int d = 0; d < D; ++d) dot = fmaf(qs[w][d], value_of<CT>(a.kv[row + d]), dot);
-      s = dot * ks * a.scale;
+      for (int d = 0; d < D; ++d) dot = fmaf(q[d], value_of<CT>(a.kv[row + d]), dot);
+      x = dot * ks * a.scale;
     }
-    const float mn = fmaxf(m, wave_max_f32_dpp(s)), ms = mn == NEG_INF ? 0.f : mn;
-    const float p = j < hi ? exp2f(s - ms) : 0.f, f = exp2f(m - ms);
-    l = l * f + wave_sum_f32_dpp(p);
+    const float mn = fmaxf(s.m, wave_max_f32_dpp(x)), ms = mn == NEG_INF ? 0.f : mn;
+    const int u = max(s.u, (int)wave_max_u32_dpp(scale_field(vs)) - 126 - 80);
+    const float p = j < hi ? exp2f(x - ms) : 0.f, f = exp2f(s.m - ms);
+    s.l = s.l * f + wave_sum_f32_dpp(p);
 #pragma unroll
-    for (int e = 0; e < ANY_D / 64; ++e) o[e] *= f;
-    const float pv = p * vs;
+    for (int e = 0; e < ANY_D / 64; ++e) s.o[e] = ldexpf(s.o[e] * f, s.u - u);
+    const float pv = p * ldexpf(vs, -u);
     for (int i = 0; i < 64 && b + i < hi; ++i) {
       const float pi = __shfl(pv, i);
       const int64_t ri = (int64_t)__shfl((long long)row, i) + D;
 #pragma unroll
       for (int e = 0; e < ANY_D / 64; ++e)
-        if (lane + 64 * e < D) o[e] = fmaf(pi, value_of<CT>(a.kv[ri + lane + 64 * e]), o[e]);
+        if (lane + 64 * e < D) s.o[e] = fmaf(pi, value_of<CT>(a.kv[ri + lane + 64 * e]), s.o[e]);
     }
-    m = mn;
+    s.m = mn;
+    s.u = u;
   }
+  return s;
+}
+// Its results; `any`: it has keys.
+__device__ __forceinline__ void write_plain(const AttendArgs& a, int64_t t, int h, const PlainRow& s, bool any) {
+  const int lane = threadIdx.x & 63;
   // (a query whose keys all score -inf: 0 / 0)
-  const float inv = hi > lo ? 1.f / l : 0.f;
+  const float inv = any ? 1.f / s.l : 0.f;
 #pragma unroll
-  for (int e = 0; e < ANY_D / 64; ++e)
-    if (lane + 64 * e < D) a.o[t * a.sot + h * a.soh + (lane + 64 * e) * a.sod] = sdc_to_half<DT>(hi > lo ? o[e] * inv : 0.f);
-  if (a.lse && lane == 0) a.lse[t * a.slt + h] = hi > lo ? (m + log2f(l)) * LN2 : NEG_INF;
+  for (int e = 0; e < ANY_D / 64; ++e) {
+    const int d = lane + 64 * e;
+    const float x = any ? ldexpf(s.o[e] * inv, s.u) : 0.f;
+    if (d < a.D) a.o[t * a.sot + h * a.soh + d * a.sod] = a.fp16 ? sdc_to_half<SDC_FP16>(x) : sdc_to_half<SDC_BF16>(x);
+  }
+  if (a.lse && lane == 0) a.lse[t * a.slt + h] = any ? (s.m + log2f(s.l)) * LN2 : NEG_INF;
+}
+
+template <int CT>
+__global__ __launch_bounds__(256) void kv_attend_any(AttendArgs a) {
+  __shared__ float qs[4][ANY_D];
+  const int w = threadIdx.x >> 6;
+  const int64_t id = (int64_t)blockIdx.x * 4 + w;
+  if (id >= a.st.T * a.Hq) return;
+  const int64_t t = id / a.Hq;
+  const int h = (int)(id - t * a.Hq);
+  plain_query(a, t, h, qs[w]);
+  Request rq;
+  int64_t first;
+  const int r = sdc_find_request(a.st, t, 1, 0, rq, first);
+  int64_t lo = 0, hi = 0;
+  if (r >= 0 && r < a.st.R) {
+    hi = min(t - rq.q1 + rq.len + 1, a.maxlen);
+    lo = max(t - rq.q1 + rq.len + 1 - a.window, (int64_t)0);
+  }
+  write_plain(a, t, h, plain_row<CT>(a, qs[w], r, h / a.G, lo, hi), hi > lo);
 }
 
 // ------------------------------------------------------------------------------------------------ few query rows
 constexpr int ROWS = 16;                       // query rows (tokens x heads of one kv head) of a tile
 constexpr int MAXP = 1024;                     // page-table entries a workgroup holds
 constexpr float M0 = -3.0e38f;                 // a maximum before the first key
+constexpr float BIAS = 13.f;                   // the largest probability is 2^BIAS .. 2^(BIAS + 2): fp16 has room under it
+constexpr int HEAD = 4;                        // numbers of a row at the start of a part's record
 
 // Four codes as two pairs of fp16, exactly.
 template <int CT>
@@ -153,6 +190,39 @@ __device__ __forceinline__ void transpose4(const uint32_t* x, uint32_t* y) {
 
 // which of the four codes are NaN (0x7F or 0xFF), as 0x80 bits
 __device__ __forceinline__ uint32_t nan_codes(uint32_t x) { return ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// The largest field of a part's value scales, and of 255 - field without the smallest scale, which pages of zeros have.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 larger(u16x2 x, uint32_t y) { return __builtin_elementwise_max(x, __builtin_bit_cast(u16x2, y)); }
+__device__ __forceinline__ u16x2 scale_ends(u16x2 x, float v) {
+  const uint32_t f = scale_field(v);
+  return larger(x, f | (f > 1 ? 255u - f : 0u) << 16);
+}
+__device__ __forceinline__ u16x2 wave_larger(u16x2 v) {
+  v = larger(v, dpp_u32<0xB1>(__builtin_bit_cast(uint32_t, v)));
+  v = larger(v, dpp_u32<0x4E>(__builtin_bit_cast(uint32_t, v)));
+  v = larger(v, dpp_u32<0x141>(__builtin_bit_cast(uint32_t, v)));
+  v = larger(v, dpp_u32<0x140>(__builtin_bit_cast(uint32_t, v)));
+  const int x = __builtin_bit_cast(int, v);
+#pragma unroll
+  for (int l = 0; l < 64; l += 16) v = larger(v, (uint32_t)__builtin_amdgcn_readlane(x, l));
+  return v;
+}
+// How a page's value scale enters the products: as 2^b times a factor in [1/2, 1).  2^(x + b), x a score, is what a probability's
+// product with its scale is rounded in, so it is that exponent whose maximum is followed; the sum of probabilities takes 2^-b of
+// it.  With b from LOW_B to HIGH_B neither loses keys to fp32's ends.  Zero, and the scale 2^-126 of a page of zeros, count as
+// 2^LOW_B, with their values next to nothing.
+constexpr int LOW_B = -60, HIGH_B = 40;
+__device__ __forceinline__ int scale_exponent(float v) {
+  const int f = (int)scale_field(v);
+  return f > 1 ? f - 126 : fabsf(v) < 1.f ? LOW_B : 0;
+}
+__device__ __forceinline__ float scale_factor(float v, int b) { return ldexpf(v, -b); }
+// Whether a part has scales outside that (values of 1e15 and more, or under 4e-16): it is left to plain_row.
+__device__ __forceinline__ bool scales_far(u16x2 ends) {
+  const int top = __builtin_amdgcn_readfirstlane(ends.x), low = __builtin_amdgcn_readfirstlane(ends.y);
+  return top > 126 + HIGH_B || top == 1 || (low && 255 - low < 126 + LOW_B);
+}
 
 // Over the lanes l, l + 16, l + 32, l + 48: rows of 16 swapped by VALU moves (a trip through LDS takes ten times as long;
 // 24 sequences with a chunk of 500 24.3 us, 26.1 so).
@@ -234,11 +304,57 @@ __device__ __forceinline__ void write_four(const AttendArgs& a, int64_t tok, int
     for (int i = 0; i < 4; ++i) o[(d + i) * a.sod] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
 }
 
+// What a row's sums come to: x (elements d .. d + 3) in units of 2^(m + up), l in units of 2^(m - bias), x too.
+__device__ __forceinline__ void write_row(const AttendArgs& a, const Tile& t, int tok, int64_t token, int head, int d, float m, float up,
+                                          float l, f32x4 x, float bias) {
+  // (a row with keys whose scores are all -inf: 0 / 0)
+  const int64_t p = t.p0 + tok;
+  const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
+  const float half = up == 0.f ? 1.f : __builtin_amdgcn_exp2f(0.5f * up);       // (2^up itself may be no fp32 number)
+  write_four(a, token, head, d, x * (any ? half / l : 0.f), half);
+  if (a.lse && d == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l) - bias) * LN2 : NEG_INF;
+}
+
 // One row's results: x[0 .. n) at elements d.., scaled.
 __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t tok, int h, int d, const float* x, int n, float f) {
   uint16_t* o = a.o + tok * a.sot + h * a.soh;
   for (int i = 0; i < n && d + i < a.D; ++i)
     o[(d + i) * a.sod] = a.fp16 ? sdc_to_half<SDC_FP16>(x[i] * f) : sdc_to_half<SDC_BF16>(x[i] * f);
+}
+
+// The workgroup's part by plain_row, a wave a row; q: ANY_D floats of LDS a wave.  The kernel's arguments are read again, and the
+// tile is found again: kept for this they would cost the callers their registers.
+template <int CT>
+__device__ __forceinline__ void plain_part(float* q, int waves) {
+  auto args = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const AttendArgs& a = *(const AttendArgs*)args;
+  const Split& sp = *(const Split*)(args + sizeof(AttendArgs));
+  static_assert(sizeof(AttendArgs) % alignof(Split) == 0, "the second argument follows the first");
+  const int lane = threadIdx.x & 63, D = a.D, w = threadIdx.x >> 6;
+  const int s = blockIdx.x % sp.S, tile = sp.rows == ROWS ? blockIdx.x / sp.S : (int)(sp.tiles - 1 - blockIdx.x / sp.S);
+  Tile t;
+  if (!find_tile(a, sp, tile, t)) return;
+  const int64_t a0 = t.c0 + (int64_t)s * t.C, a1 = min(t.khi, a0 + t.C);
+  q += w * ANY_D;
+  for (int row = w; row < sp.GB * sp.TB; row += waves) {
+    const int tok = row / sp.GB, hd = t.hb * sp.GB + row % sp.GB;
+    if (tok >= t.ntok || hd >= a.G) continue;
+    const int64_t p = t.p0 + tok, token = t.tok0 + tok, lo = max(p - a.window + 1, a0), hi = min(min(p + 1, a.maxlen), a1);
+    const int head = t.hk * a.G + hd;
+    plain_query(a, token, head, q);
+    const PlainRow r = plain_row<CT>(a, q, t.r, t.hk, lo, hi);
+    if (t.nsp == 1) {
+      write_plain(a, token, head, r, hi > lo);
+      continue;
+    }
+    float* rec = sp.part + ((int64_t)tile * sp.S + s) * sp.rows * (D + HEAD);
+    const float m = fmaxf(r.m, M0);
+    if (lane == 0) *reinterpret_cast<f32x4*>(rec + HEAD * row) = f32x4{m + (float)r.u, m, r.l, 0.f};
+#pragma unroll
+    for (int e = 0; e < ANY_D / 64; ++e)
+      if (lane + 64 * e < D) rec[HEAD * sp.rows + row * D + lane + 64 * e] = r.o[e];
+  }
 }
 
 // Tiles of up to 16 query rows over a part of their keys: HBM bound, so a wave streams 32 keys at a time straight into
@@ -248,24 +364,26 @@ __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t tok, int 
 // other lane; V^T's fragments are 4 x 4 byte transposes of rows that a lane reads DP / 16 codes of.  Codes are exact in
 // fp16; queries are scaled to it by a power of two per row (a bf16 element 2^-27 of its row's largest keeps all bits).
 // The key scales multiply the scores, the value scales the probabilities, in fp32.  Probabilities are rounded to fp16's
-// 11 bits, in units that put their largest product with a value scale at 2^13 .. 2^15.
+// 11 bits, in units that put their largest product with a value scale at 2^12 .. 2^15 (scale_exponent).
 // Four sequences of 100-131k tokens, 8 heads of 128: 173 us, 5.6 TB/s; 64 of 512-2048 tokens 37 us; one of 500 11 us.
 template <int CT, int DP, int PN>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendArgs a, Split sp) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) void kv_attend_rows(AttendArgs a, Split sp) {
   constexpr int NW = 4, KEYS = 32 * NW;                     // keys that the workgroup's waves take at a time
   constexpr int KW = DP / 64;                  // 16-byte reads of a key per lane; dwords of a value per lane
   constexpr int NS = DP / 32, ND = DP / 16;    // depth steps of a score, row blocks of the output
   constexpr int QS = DP + 8, OS = DP + 4;      // row pitches in LDS
   struct Head {
-    float2 sc[MAXP];
+    float2 ks[MAXP], vs[MAXP];                 // of each page: ks and b; 2^-b and the factor on 2^b (in [1/2, 1) mostly)
     int32_t pg[MAXP];
     _Float16 q[ROWS][QS];
   };
   __shared__ union {
     Head h;
     float o[NW][ROWS][OS];
+    float plain[NW][ANY_D];
   } sh;
-  __shared__ float rowf[ROWS], wmax[NW], ml[NW][ROWS][2];
+  __shared__ float rowf[ROWS], ml[NW][ROWS][2];
+  __shared__ u16x2 wends[NW];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = a.D, N = a.st.N;
@@ -378,7 +496,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
   };
 
   // the pages' scales, then the first codes: a wait for the former leaves the latter on their way
-  float vmax = 0.f;
+  u16x2 ends = {0, 0};
   Buf b0, b1;
   int k = 32 * w;
   float2 sc0 = {0.f, 0.f};
@@ -394,10 +512,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
     float2 sc = sc0;
     if (i != tid) sc = {scp[0], scp[1]};
     if (page < 0) sc = {__builtin_nanf(""), __builtin_nanf("")};
-    sh.h.sc[i] = sc;
-    const float v = fabsf(sc.y);
-    if (v <= 3.0e38f) vmax = fmaxf(vmax, v);
+    const int b = scale_exponent(sc.y);
+    sh.h.ks[i] = {sc.x, (float)b};
+    sh.h.vs[i] = {ldexpf(1.f, -b), scale_factor(sc.y, b)};
+    ends = scale_ends(ends, sc.y);
   }
+  ends = wave_larger(ends);
+  if (lane == 0) wends[w] = ends;
   {
     float x[ND], amax = 0.f;
     if (a.fp16) {
@@ -428,15 +549,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
       if (tid < 256) sh.h.q[orow][od + i] = (_Float16)(x[i] * f);
     if (tid < 256 && (tid & 15) == 0) rowf[orow] = ldexpf(a.scale, e - 13);
   }
-  vmax = wave_max_f32_dpp(vmax);
-  if (lane == 0) wmax[w] = vmax;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NW; ++i) vmax = fmaxf(vmax, wmax[i]);
-  int ve;
-  (void)frexpf(vmax, &ve);
-  const int bias = 13 - min(max(ve, -100), 100);                        // probabilities in units of 2^-bias
-  const float fbias = (float)bias, unit = ldexpf(1.f, -bias);
+  for (int i = 0; i < NW; ++i) ends = __builtin_elementwise_max(ends, wends[i]);
+  if (scales_far(ends)) {
+    __syncthreads();                           // (the tables' place is the plain rows')
+    plain_part<CT>(&sh.plain[0][0], NW);
+    return;
+  }
   f16x8 qf[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) qf[i] = *reinterpret_cast<const f16x8*>(&sh.h.q[c][g * (DP / 4) + 8 * i]);
@@ -471,13 +591,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
         sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8<CT>(b.k[u][i / 2][2 * (i % 2)], b.k[u][i / 2][2 * (i % 2) + 1]),
                                                        qf[i], sc[u], 0, 0, 0);
     }
+    // With b the exponent of the page's value scale, p v is 2^(x + b) times a factor of at most 1: it is that exponent whose
+    // maximum m is, and the sum of probabilities takes 2^-b of it.
     float x[8], top = M0;
     float2 ps[8];                              // the keys' scales
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ps[j] = sh.h.sc[b.e[j]];
+    for (int j = 0; j < 8; ++j) ps[j] = sh.h.ks[b.e[j]];
     const bool edge = k0 < flo || k0 + 32 > fhi;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = sc[j / 4][j % 4] * (ps[j].x * rf);
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(sc[j / 4][j % 4], ps[j].x * rf, ps[j].y);
     bool seen[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) seen[j] = true;
@@ -491,7 +613,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
-    // the maximum follows the scores only when they pass it by 2 (a factor of 4, which fp16 has room for)
+    // the maximum follows only when it is passed by 2 (a factor of 4, which fp16 has room for)
     if (__any(top > m + 2.f)) {
       const float mn = fmaxf(m, over_groups_max(top));
       const float f = exp2f(m - mn);
@@ -500,11 +622,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
       for (int n = 0; n < ND; ++n) o[n] *= f;
       m = mn;
     }
+    const float down = BIAS - m;
     float p[8];
 #pragma unroll
+    for (int j = 0; j < 8; ++j) ps[j] = sh.h.vs[b.e[j]];
+#pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(x[j] - m + fbias);
-      l += p[j];
+      p[j] = __builtin_amdgcn_exp2f(x[j] + down);
+      l = fmaf(p[j], ps[j].x, l);
       p[j] *= ps[j].y;
     }
     if (edge) {
@@ -606,18 +731,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void kv_attend_rows(AttendAr
       x += f * *reinterpret_cast<const f32x4*>(&sh.o[u][row][d]);
     }
     if (t.nsp == 1) {
-      // (a row with keys whose scores are all -inf: 0 / 0)
-      const int64_t p = t.p0 + tok;
-      const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-      write_four(a, token, head, d, x, any ? 1.f / lt : 0.f);
-      if (a.lse && d == 0) a.lse[token * a.slt + head] = any ? (mt + log2f(lt) - fbias) * LN2 : NEG_INF;
+      write_row(a, t, tok, token, head, d, mt, 0.f, lt, x, BIAS);
     } else {
-      float* rec = sp.part + (int64_t)blockIdx.x * ROWS * (D + 2);
-      if (d == 0) {
-        rec[2 * row] = mt;
-        rec[2 * row + 1] = lt * unit;
-      }
-      *reinterpret_cast<f32x4*>(rec + 2 * ROWS + row * D + d) = x * unit;
+      float* rec = sp.part + (int64_t)blockIdx.x * ROWS * (D + HEAD);
+      constexpr float unit = 0x1p-13f;         // 2^-BIAS
+      if (d == 0) *reinterpret_cast<f32x4*>(rec + HEAD * row) = f32x4{mt, mt, lt * unit, 0.f};
+      *reinterpret_cast<f32x4*>(rec + HEAD * ROWS + row * D + d) = x * unit;
     }
   }
 }
@@ -666,7 +785,6 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   constexpr int KC = DP == 96 ? 8 : DP / 16, KU = (KT * KC + HT - 1) / HT;
   constexpr int VC = DP <= 96 ? 32 : DP / 4, VUN = KT / 8 * VC, VU = (VUN + HT - 1) / HT;
   constexpr int NX = 4 * KU > 8 * VU ? 4 * KU : 8 * VU;
-  constexpr float BIAS = 13.f;
   struct Stage {
     uint8_t k[KT * KP];
     uint8_t v[4 * VR * VP];
@@ -1123,12 +1241,9 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     each([&](int d, f32x4 x) { write_four(a, r.token, r.head, d, x, f); });
     if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = any ? (m + log2f(l) - BIAS) * LN2 : NEG_INF;
   } else {
-    float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + 2);
-    if (h == 0) {
-      rec[2 * r.row] = m;
-      rec[2 * r.row + 1] = l * 0x1p-13f;
-    }
-    each([&](int d, f32x4 x) { *reinterpret_cast<f32x4*>(rec + 2 * TALL + r.row * D + d) = x * 0x1p-13f; });
+    float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + HEAD);
+    if (h == 0) *reinterpret_cast<f32x4*>(rec + HEAD * r.row) = f32x4{m, m, l * 0x1p-13f, 0.f};
+    each([&](int d, f32x4 x) { *reinterpret_cast<f32x4*>(rec + HEAD * TALL + r.row * D + d) = x * 0x1p-13f; });
   }
 }
 
@@ -1165,42 +1280,40 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a, Split rows, 
   if (t.nsp < 2) return;
   const int row = tok * sp.GB + hd - t.hb * sp.GB;
   first = sp.slots ? (int64_t)t.r * sp.slots : (int64_t)((uint32_t)a.st.qsl[t.r] / (uint32_t)sp.TB) + t.r;
-  const int64_t tile = ((first + tt) * a.Hkv + t.hk) * sp.NHB + t.hb, size = (int64_t)sp.rows * (D + 2);
+  const int64_t tile = ((first + tt) * a.Hkv + t.hk) * sp.NHB + t.hb, size = (int64_t)sp.rows * (D + HEAD);
   const float* rec = sp.part + tile * sp.S * size;
   if (head >= a.Hq || d >= D) return;
-  const float* ml = rec + 2 * row;
-  const float* v = rec + 2 * sp.rows + row * D + d;
-  float m = M0, l = 0.f;
+  const float* begin = rec + HEAD * row;
+  const float* v = rec + HEAD * sp.rows + row * D + d;
+  float m = M0, ml = M0, l = 0.f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
   constexpr int U = 4;                         // parts whose loads are on their way at once
   for (int b = 0; b < t.nsp; b += U) {
-    float2 w[U];
-    f32x4 y[U];
+    f32x4 w[U], y[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int64_t at = min(b + i, t.nsp - 1) * size;
-      w[i] = *reinterpret_cast<const float2*>(ml + at);
+      w[i] = *reinterpret_cast<const f32x4*>(begin + at);
       y[i] = *reinterpret_cast<const f32x4*>(v + at);
     }
-    float mn = m;
+    float mn = m, mln = ml;
 #pragma unroll
-    for (int i = 0; i < U; ++i) mn = fmaxf(mn, w[i].x);
-    const float f = __builtin_amdgcn_exp2f(m - mn);
-    l *= f;
-    x *= f;
+    for (int i = 0; i < U; ++i) {
+      mn = fmaxf(mn, w[i][0]);
+      mln = fmaxf(mln, w[i][1]);
+    }
+    x *= __builtin_amdgcn_exp2f(m - mn);
+    l *= __builtin_amdgcn_exp2f(ml - mln);
     m = mn;
+    ml = mln;
 #pragma unroll
     for (int i = 0; i < U; ++i)
       if (b + i < t.nsp) {
-        const float g = __builtin_amdgcn_exp2f(w[i].x - m);
-        l = fmaf(g, w[i].y, l);
-        x += g * y[i];
+        x += __builtin_amdgcn_exp2f(w[i][0] - m) * y[i];
+        l = fmaf(__builtin_amdgcn_exp2f(w[i][1] - ml), w[i][2], l);
       }
   }
-  const int64_t p = t.p0 + tok;
-  const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-  write_four(a, token, head, d, x, any ? 1.f / l : 0.f);
-  if (a.lse && d == 0) a.lse[token * a.slt + head] = any ? (m + log2f(l)) * LN2 : NEG_INF;
+  write_row(a, t, tok, token, head, d, ml, m - ml, l, x, 0.f);
 }
 
 // The tiles and parts of a call, from its sizes alone.
@@ -1266,7 +1379,7 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
   }
   return p;
 }
-int64_t part_bytes(const Split& sp, int64_t D) { return sp.S <= 1 ? 0 : sp.tiles * sp.S * sp.rows * (D + 2) * 4; }
+int64_t part_bytes(const Split& sp, int64_t D) { return sp.S <= 1 ? 0 : sp.tiles * sp.S * sp.rows * (D + HEAD) * 4; }
 
 int launch_join(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   if (p.rows.S == 1 && p.tiles.S <= 1) return SDC_OK;
@@ -1316,15 +1429,12 @@ int run_tiles(const AttendArgs& a, const Split& sp, hipStream_t stream) {
   return a.D <= 128 ? launch_tiles<CT, 128>(a, sp, stream) : launch_tiles<CT, 256>(a, sp, stream);
 }
 
-template <int DT>
 int run(int cache, const AttendArgs& a, hipStream_t stream) {
   const int64_t blocks = sdc_cdiv(a.st.T * a.Hq, 4);
   if (blocks > 0x7FFFFFFF) return SDC_EUNSUPPORTED;
   SdcProf prof("kv_attend", stream);
-  if (cache == SDC_CACHE_E4M3)
-    hipLaunchKernelGGL((kv_attend_any<DT, SDC_CACHE_E4M3>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((kv_attend_any<DT, SDC_CACHE_I8>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  if (cache == SDC_CACHE_E4M3) hipLaunchKernelGGL((kv_attend_any<SDC_CACHE_E4M3>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((kv_attend_any<SDC_CACHE_I8>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
   SDC_LAUNCH_CHECK();
   return SDC_OK;
 }
@@ -1378,5 +1488,5 @@ extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, i
       rc = cache == SDC_CACHE_E4M3 ? run_rows<SDC_CACHE_E4M3>(a, p.rows, stream) : run_rows<SDC_CACHE_I8>(a, p.rows, stream);
     return rc == SDC_OK ? launch_join(a, p, stream) : rc;
   }
-  return dtype == SDC_BF16 ? run<SDC_BF16>(cache, a, stream) : run<SDC_FP16>(cache, a, stream);
+  return run(cache, a, stream);
 }
