@@ -6,7 +6,7 @@
 //
 // kv_attend_rows: tiles of 16 query rows, for decode steps and small chunks (HBM bound, or by latency).  kv_attend_tiles:
 // tiles of 256 query rows, for chunks of a prompt (bound by the matrix cores and the softmax between them).  kv_attend_any:
-// any head size and alignment, a row a wave; kv_attend_rows leaves a part whose value scales are far from 1 to the same (plain_row).
+// any head size and alignment, a row a wave; parts whose value scales are far from 1 are left to the same (plain_row).
 // A part of a tile's keys is one workgroup's; kv_attend_join joins the parts in their order.
 #include <algorithm>
 #include <type_traits>
@@ -767,8 +767,7 @@ __device__ __forceinline__ float over_halves_sum(float v) {
 // y = x + log2 vs the product p vs is 2^(y - m): one fused multiply-add and one exponential a score, while the next tile's
 // scores are computed.  m follows the largest y, and the sum takes the group's sum over vs.  Scales without a logarithm are
 // factors on the widened values; keys that a row does not see score -inf; values of NaN under a tile that some row sees only
-// in part are left out and put in at the end.  Rounding of the probabilities and their units: as kv_attend_rows (values whose
-// scale is under 2^-90 lose bits).
+// in part are left out and put in at the end.  Rounding of the probabilities, and scales far from 1: as kv_attend_rows.
 //
 // Two chunks of 2048 tokens behind up to 3000 keys, 32 heads of 128: 285 us, 890 TFLOP/s; the matrix cores are busy 38 % of
 // it, LDS 27 %.  Waves of 32 rows: 64 would need all 512 registers, 16 twice the fragments.
@@ -790,7 +789,12 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     uint8_t v[4 * VR * VP];
     float4 sc[KT];                             // of each key, as of its page
   };
+  struct WaveScales {
+    u16x2 ends;
+    bool flip, mul;
+  };
   __shared__ Stage st[2];
+  __shared__ WaveScales wscales[NW];
   __shared__ int32_t pg[MAXP];
   __shared__ float4 ps[MAXP];                  // of each page: |ks|, log2 vs, 1 / vs, the factor on the stored values
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
@@ -833,6 +837,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   f16x8 qf[NS];
   float rf;
   bool flip = false, mul = false;
+  u16x2 ends = {0, 0};
   int64_t prow;                                // the lane's position
   {
     const Row r = row_of();
@@ -855,17 +860,19 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     }
     int e = 0;
     // The part's pages and their scales.  A page outside the cache is page 0 with scales of NaN.  Value scales that have no
-    // logarithm (0, infinity, NaN) become factors on the widened values, and so do signs; a key scale of NaN makes the page's
-    // share of the sum and its values NaN.
+    // logarithm (infinity, NaN) become factors on the widened values, and so do signs and what scales under 2^LOW_B are less
+    // than that; a key scale of NaN makes the page's share of the sum and its values NaN.
     for (int i = tid; i < np; i += 2 * HT) {
       const int32_t p = a.st.bt[t.r * a.st.sbt + fp + i];
       const bool in = p >= 0 && p < a.st.NB;
       const float* scp = a.scales + (in ? (int64_t)p : 0) * a.sb + t.hk * a.sh;
       const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf(""), v = fabsf(vs);
-      const bool log = v > 0.f && v < __builtin_inff(), key = ks == ks;
-      ps[i] = {key ? fabsf(ks) : 0.f, log ? log2f(v) : 0.f, !key ? ks : log ? fminf(1.f / v, 0x1p126f) : 1.f,
-               !key ? ks : !log ? vs : vs < 0.f ? -1.f : 1.f};
+      const bool log = scale_field(v) > 1, small = v < 0x1p-125f, key = ks == ks;
+      const float inv = log ? 1.f / v : small ? ldexpf(1.f, -LOW_B) : 1.f;
+      ps[i] = {key ? fabsf(ks) : 0.f, log ? log2f(v) : small ? (float)LOW_B : 0.f, !key ? ks : inv,
+               !key ? ks : log ? (vs < 0.f ? -1.f : 1.f) : vs * inv};
       pg[i] = (in ? p : 0) | (ks < 0.f ? (int32_t)0x80000000 : 0);        // the sign of ks, which the keys take
+      ends = scale_ends(ends, vs);
       flip |= ks < 0.f;
       mul |= !log || vs < 0.f || !key;
     }
@@ -894,7 +901,23 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     else narrow(std::integral_constant<int, SDC_BF16>{});
     rf = ldexpf(fabsf(a.scale), e - 13);       // (scores times key scales that are not negative keep their order)
   }
-  const bool flips = __syncthreads_or(flip), muls = __syncthreads_or(mul);      // (which is 0 or 1, not the values' or)
+  ends = wave_larger(ends);
+  const bool wave_flip = __any(flip), wave_mul = __any(mul);
+  if (lane == 0) wscales[w] = {ends, wave_flip, wave_mul};
+  __syncthreads();
+  flip = mul = false;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const WaveScales x = wscales[i];
+    ends = __builtin_elementwise_max(ends, x.ends);
+    flip |= x.flip;
+    mul |= x.mul;
+  }
+  const bool flips = __builtin_amdgcn_readfirstlane(flip), muls = __builtin_amdgcn_readfirstlane(mul);
+  if (scales_far(ends)) {
+    plain_part<CT>(reinterpret_cast<float*>(st), NW);
+    return;
+  }
   // keys, counted from a0: those of the tile; those that the lane's row sees; those that a row of the wave, and every row of
   // the wave sees; those that every row of the tile sees
   auto clip = [](int64_t x) { return (int)max(min(x, (int64_t)1 << 30), -((int64_t)1 << 30)); };
@@ -1111,7 +1134,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       float z = x[j0 / 16][j0 % 16];
 #pragma unroll
       for (int i = 1; i < GE; ++i) z = fmaxf(z, x[(j0 + i) / 16][(j0 + i) % 16]);
-      top = fmaxf(top, fmaf(z, factor(sc.x), fmaxf(sc.y, -90.f)));
+      top = fmaxf(top, fmaf(z, factor(sc.x), sc.y));
     }
     // the maximum follows the scores when they pass it by 2 (fp16 has room for that)
     if (__any(top > m + 2.f)) {
@@ -1123,9 +1146,11 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       m = mn;
     }
     f16x8 pf[KT / 16];
+    // (keys that share no page: their scales are read where they are used, 128 registers would not hold them)
+    constexpr bool EACH = GE == 1;
     float cs[NG], b0[NG], inv[NG], sum[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
+    for (int g = 0; g < (EACH ? 0 : NG); ++g) {
       const float4 sc = scales(g * GE);
       cs[g] = factor(sc.x);
       b0[g] = sc.y - m + BIAS;
@@ -1145,15 +1170,22 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
 #pragma unroll
         for (int j = q * 16 * KB / MK; j < (q + 1) * 16 * KB / MK; ++j) {
           const int g = j / GE;
-          const float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs[g], b0[g]));
-          sum[g] += p;
+          float p;
+          if constexpr (EACH) {
+            const float4 sc = scales(j);
+            p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], factor(sc.x), sc.y - m + BIAS));
+            l = p == 0.f ? l : fmaf(p, sc.z, l);
+          } else {
+            p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], cs[g], b0[g]));
+            sum[g] += p;
+          }
           pf[j / 8][j % 8] = (_Float16)p;
         }
       }
       __builtin_amdgcn_sched_barrier(0x6);
     }
 #pragma unroll
-    for (int g = 0; g < NG; ++g) l = sum[g] == 0.f ? l : fmaf(sum[g], inv[g], l);
+    for (int g = 0; g < (EACH ? 0 : NG); ++g) l = sum[g] == 0.f ? l : fmaf(sum[g], inv[g], l);
   };
 
   // In the step of tile t the waves take the values of t and the keys of t + 1.  At its start the values of t + 1 and the keys of

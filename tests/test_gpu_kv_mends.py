@@ -4,12 +4,12 @@ from __future__ import annotations
 
 import math
 
-import numpy as np
 import pytest
 import torch
 
 from oracle import paged
-from tests.test_gpu_kv_attn import DEV, append_checked, attend_checked, make, step, stood_for
+from sdcguard_amd import _lib
+from tests.test_gpu_kv_attn import DEV, append_checked, attend_checked, make, step
 
 pytestmark = pytest.mark.gpu
 
@@ -45,26 +45,66 @@ def test_append_of_the_largest_finite_values(layout, N, kind):
             assert math.copysign(1.0, float(x)) == math.copysign(1.0, float(codes[at, h, slot, d]))
 
 
+def plain64(c):
+    """(o, lse, mass, top, terms) of the step's queries in float64 on the device: the outputs, sum p |v| / sum p, the same with
+    each value its scale's largest, and the largest |q| . |k| scale of a row.  (Finite caches, no window.)"""
+    D, N, Hkv = c["D"], c["N"], c["kv"].shape[1]
+    code = c["kv"].view(torch.uint8).view(c["kv"].dtype).float().double()
+    sc = c["scales"].double()
+    outs = []
+    for r, n in enumerate(c["lens"].tolist()):
+        a, b = int(c["qsl"][r]), int(c["qsl"][r + 1])
+        pages = c["bt"][r, :-(-n // N)].long()
+        x = code[pages].transpose(1, 2).reshape(-1, Hkv, 2 * D)[:n]              # (keys, kv heads, 2 D)
+        ks, vs = sc[pages].repeat_interleave(N, 0)[:n].unbind(-1)
+        q = c["q"][a:b].double().view(b - a, Hkv, -1, D)
+        k, v = x[..., :D] * ks[..., None], x[..., D:] * vs[..., None]
+        s = torch.einsum("thgd,khd->thgk", q, k) * D ** -0.5
+        terms = torch.einsum("thgd,khd->thgk", q.abs(), k.abs()).amax(-1) * D ** -0.5
+        seen = torch.arange(n, device=DEV) <= torch.arange(n - (b - a), n, device=DEV)[:, None]
+        s = s.masked_fill(~seen[:, None, None], float("-inf"))
+        p = torch.softmax(s, -1)
+        flat = [torch.einsum("thgk,khd->thgd", p, y) for y in (v, v.abs(), vs[..., None].abs() * paged.TOP[c["kind"]])]
+        outs.append([y.flatten(1, 2) for y in (flat[0], torch.logsumexp(s, -1), flat[1], flat[2], terms)])
+    return [torch.cat(y) for y in zip(*outs)]
+
+
 def attend_tight(c, **kw):
     """attend_checked with a bound that only the keys which a row sees, at their weights, have a part in."""
     from sdcguard_amd.kv_attn import kv_attend
     o, lse = kv_attend(c["q"], c["kv"], c["scales"], *step(c), return_lse=True, **kw)
-    D, T, kv = c["D"], c["T"], stood_for(c["kv"], c["scales"])
-    case = (c["qsl"].tolist(), c["lens"].tolist(), c["bt"].cpu().numpy(), c["N"], D ** -0.5)
-    q = c["q"][:T].double().cpu().numpy()
-    ro, rl, mass, terms = paged.attend(q, kv, *case)
-    kv[..., D:] = c["scales"].double().abs().cpu().numpy()[:, :, None, 1:] * paged.TOP[c["kind"]]
-    top = paged.attend(q, kv, *case)[0]
-    n = int(c["lens"].max())
+    D, T, n, info = c["D"], c["T"], int(c["lens"].max()), torch.finfo(c["dt"])
+    ro, rl, mass, top, terms = plain64(c)
     ds = (D + 16) * 2.0 ** -24 * terms + 2.0 ** -20
-    # a probability's product with its scale is rounded to 11 bits, or by a fp16 step of 2^-24 where the row's largest product
-    # is 2^4 or more; a maximum of up to 2^8 that carries the scales' exponent is rounded to 2^-16
-    got, gl = o[:T].double().cpu().numpy(), lse[:T].double().cpu().numpy()
-    tol = torch.finfo(c["dt"]).eps / 2 * abs(ro) + (2.0 ** -11 + 2.0 ** -15 + 2 * ds[..., None] + (n + 16) * 2.0 ** -23) * mass \
-        + n * 2.0 ** -29 * top
-    err = abs(got - ro)
-    assert (err <= tol).all(), (np.argwhere(~(err <= tol))[:5], err[~(err <= tol)][:5], tol[~(err <= tol)][:5])
-    assert (abs(gl - rl) <= ds + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * abs(rl) + 2.0 ** -16).all(), abs(gl - rl).max()
+    # the output's rounding, of a subnormal one by half the type's smallest step; a probability's product with its scale is
+    # rounded to 11 bits, or by a fp16 step of 2^-24 where the row's largest product is 2^4 or more; a maximum of up to 2^8
+    # that carries the scales' exponent is rounded to 2^-16
+    tol = info.eps / 2 * ro.abs() + info.smallest_normal * info.eps / 2 \
+        + (2.0 ** -11 + 2.0 ** -15 + 2 * ds[..., None] + (n + 16) * 2.0 ** -23) * mass + n * 2.0 ** -29 * top
+    err = (o[:T].double() - ro).abs()
+    assert (err <= tol).all(), (int((~(err <= tol)).sum()), (~(err <= tol)).nonzero()[:5], err[~(err <= tol)][:5], tol[~(err <= tol)][:5])
+    bad = ~((lse[:T].double() - rl).abs() <= ds + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * rl.abs() + 2.0 ** -16)
+    assert not bad.any(), (bad.nonzero()[:5], lse[:T][bad][:5], rl[bad][:5])
+
+
+def tall(c):
+    """The step with so wide a table that its chunks are taken in tiles of 256 rows, and whether they were."""
+    R, W = c["bt"].shape
+    wide = torch.full((R, max(W, 2000000 // c["N"])), -7, dtype=torch.int32, device=DEV)
+    wide[:, :W] = c["bt"]
+    return {**c, "bt": wide}
+
+
+class launches:
+    """How often a kernel was launched, by name."""
+    def __enter__(self):
+        _lib.lib().sdc_profile_reset()
+        _lib.lib().sdc_profile_enable(1)
+        return lambda name: _lib.profile_read(name)[1]
+
+    def __exit__(self, *a):
+        _lib.lib().sdc_profile_enable(0)
+        _lib.lib().sdc_profile_reset()
 
 
 STEPS = (((700, 1), (40, 1)), ((700, 50), (90, 90)), ((9000, 1), (300, 1)))
@@ -100,6 +140,46 @@ def test_attention_of_value_scales_far_from_each_other(lens, N):
         c["kv"].view(torch.uint8)[at, :, :, :64], c["scales"][at, :, 0] = 0xF0, 1.0
         attend_tight(c)                                # (scores of -1000 there: no weight at all)
         c["scales"][..., 0] = ks
+    c["scales"][pages, :, 1] = (2.0 ** torch.linspace(-80, 80, pages.numel(), device=DEV))[:, None]
+    attend_tight(c)
+    c["scales"][pages, :, 1] = c["scales"][pages.flip(0), :, 1].clone()
+    attend_tight(c)
+
+
+TALL = (((700, 200), (90, 90)), ((9000, 70), (300, 1)))
+
+
+@pytest.mark.parametrize("lens", TALL, ids=["chunk", "split"])
+@pytest.mark.parametrize("D,N", [(64, 16), (128, 8), (256, 16)])
+def test_chunks_weigh_keys_whose_values_are_zeros(D, N, lens):
+    """Pages of zeros have the smallest scale, 2^-126: their keys take their part of the weights all the same, beside values of
+    ordinary and of large scales."""
+    c = tall(make(lens, D=D, Hq=4, Hkv=1, N=N, seed=23, garbage=False))
+    pages = c["bt"][0, :lens[0][0] // N].long()
+    c["kv"].view(torch.uint8)[pages[1::2], :, :, D:] = 0
+    with launches() as count:
+        for ordinary in (2.0 ** -7, 1.0, 2.0 ** 20, 2.0 ** 39):
+            c["scales"][pages, :, 1] = ordinary
+            c["scales"][pages[1::2], :, 1] = 2.0 ** -126
+            attend_tight(c)
+            c["scales"][pages[1::2], :, 0] *= 0.5      # (weights mostly under 2^-13 of the largest, of many keys)
+            attend_tight(c)
+            c["scales"][pages[1::2], :, 0] *= 2.0
+        assert count("kv_attend_tiles") == 8
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("lens", TALL, ids=["chunk", "split"])
+def test_chunks_of_value_scales_at_both_ends_and_far_from_each_other(lens, kind):
+    c = tall(make(lens, D=64, Hq=4, Hkv=1, seed=24, kind=kind, garbage=False))
+    pages = c["bt"][0, :lens[0][0] // 16].long()
+    for e in (-126, -110, -60, -24, 24, 60, 100, 118):
+        c["scales"][..., 1] = 2.0 ** e
+        attend_tight(c)
+    for last in (0, 20, 60, 100):
+        c["scales"][pages, :, 1] = 2.0 ** -30
+        c["scales"][pages[-2:], :, 1] = 2.0 ** last
+        attend_tight(c)
     c["scales"][pages, :, 1] = (2.0 ** torch.linspace(-80, 80, pages.numel(), device=DEV))[:, None]
     attend_tight(c)
     c["scales"][pages, :, 1] = c["scales"][pages.flip(0), :, 1].clone()
