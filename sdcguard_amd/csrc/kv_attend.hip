@@ -1127,13 +1127,22 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     auto scales = [&](int j0) { return scp[PN == 16 ? 2 * j0 : 32 * (j0 / 16) + 8 * (j0 % 16 / 4) + j0 % 4]; };
     auto factor = [&](float ks) { return fmaxf(ks * rf, 0x1p-126f); };  // (not 0: -inf stays)
     float top = NEG_INF;
+    auto largest = [&](int j0) {
+      float z = x[j0 / 16][j0 % 16];
+#pragma unroll
+      for (int i = 1; i < GE; ++i) z = fmaxf(z, x[(j0 + i) / 16][(j0 + i) % 16]);
+      return z;
+    };
+    if (muls) {                                // (a key scale of NaN, however little its keys would weigh)
+      asm volatile("");
+#pragma unroll
+      for (int g = 0; g < NG; ++g) l = scales(g * GE).z != scales(g * GE).z && largest(g * GE) > NEG_INF ? __builtin_nanf("") : l;
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const int j0 = g * GE;
       const float4 sc = scales(j0);
-      float z = x[j0 / 16][j0 % 16];
-#pragma unroll
-      for (int i = 1; i < GE; ++i) z = fmaxf(z, x[(j0 + i) / 16][(j0 + i) % 16]);
+      const float z = largest(j0);
       top = fmaxf(top, fmaf(z, factor(sc.x), sc.y));
     }
     // the maximum follows the scores when they pass it by 2 (fp16 has room for that)

@@ -184,3 +184,19 @@ def test_chunks_of_value_scales_at_both_ends_and_far_from_each_other(lens, kind)
     attend_tight(c)
     c["scales"][pages, :, 1] = c["scales"][pages.flip(0), :, 1].clone()
     attend_tight(c)
+
+
+@pytest.mark.parametrize("N", [16, 8, 6])
+@pytest.mark.parametrize("large", [False, True])
+def test_keys_that_are_nan_reach_lse_too(large, N):
+    """A page outside the cache, and one whose key scale is NaN: where the other keys score hundreds more as well."""
+    c = make(((300, 200), (90, 1)), D=64, Hq=4, Hkv=2, N=N, seed=25, garbage=False)
+    c["bt"][0, 150 // N] = -1
+    c["scales"][c["bt"][1, 1].long(), 1, 0] = float("nan")
+    for scale in (None, 10.0, 300.0):
+        with launches() as count:
+            o, lse = attend_checked(tall(c) if large else c, scale=scale)
+            assert count("kv_attend_tiles") == int(large)
+        first = 150 // N * N - 100                     # the first row that sees the page
+        assert lse[first:200].isnan().all() and not lse[:first].isnan().any()
+        assert lse[200, 2:].isnan().all() and not lse[200, :2].isnan().any()
