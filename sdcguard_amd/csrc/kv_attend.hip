@@ -537,7 +537,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) voi
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       const float f = fabsf(x[i]);
-      if (f <= 3.3e38f) amax = fmaxf(amax, f);
+      if (f < __builtin_inff()) amax = fmaxf(amax, f);
     }
     amax = row_max(amax);
     int e = 0;
@@ -883,7 +883,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x = fabsf(lo_of<DT>(raw[i][j])), y = fabsf(hi_of<DT>(raw[i][j]));
-          amax = fmaxf(amax, fmaxf(x <= 3.3e38f ? x : 0.f, y <= 3.3e38f ? y : 0.f));
+          amax = fmaxf(amax, fmaxf(x < __builtin_inff() ? x : 0.f, y < __builtin_inff() ? y : 0.f));
         }
       amax = over_halves_max(amax);
       (void)frexpf(amax, &e);

@@ -200,3 +200,13 @@ def test_keys_that_are_nan_reach_lse_too(large, N):
         first = 150 // N * N - 100                     # the first row that sees the page
         assert lse[first:200].isnan().all() and not lse[:first].isnan().any()
         assert lse[200, 2:].isnan().all() and not lse[200, :2].isnan().any()
+
+
+@pytest.mark.parametrize("large", [False, True])
+def test_queries_up_to_the_largest_number(large):
+    """bf16's largest numbers are queries like others."""
+    c = make(((300, 200), (90, 1)), D=64, Hq=4, Hkv=1, seed=26, garbage=False)
+    c["scales"][..., 0] = 2.0 ** -132                  # (scores of a few units)
+    c["q"][:, :, 5] = torch.finfo(torch.bfloat16).max
+    c["q"][1::2, :, 5] *= -1.0
+    attend_tight(tall(c) if large else c)
