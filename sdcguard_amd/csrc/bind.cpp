@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <string>
 
@@ -65,6 +66,15 @@ bool truth(PyObject* o) {
   if (v < 0) throw Raised{};
   return v != 0;
 }
+
+// The cache's operators, and a rotation's frequencies, have no gradient: rather than drop one the call is refused.
+void no_gradient(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad())
+      value_error(std::string(what) + " takes no gradient: detached tensors, or torch.no_grad(), are needed");
+}
+const Tensor* get(const Maybe& t) { return t ? &*t : nullptr; }
 
 int half_code(const Tensor& t) {
   if (t.scalar_type() == at::kBFloat16) return 0;
@@ -168,6 +178,7 @@ PyObject* rotate(PyObject* const* a) {
   const How how{truth(a[3]), truth(a[5]), number(a[4])};
   const Maybe out = maybe(a[6], "out");
   if (x.dim() < 3) value_error("x must be (..., tokens, heads, head size)");
+  no_gradient("turns", {&turns});
   const at::Device dev = x.device();
   check_turns(turns, x.size(-1), dev);
   const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 2);
@@ -244,6 +255,7 @@ PyObject* append(PyObject* const* a) {
   Maybe positions = maybe(a[8], "positions"), out = maybe(a[12], "query_out");
   const bool interleaved = truth(a[9]);
   const double mscale = number(a[10]);
+  no_gradient("kv_append", {&key, &value, &kv, get(scales), get(turns), get(query), get(out)});
   const at::Device dev = key.device();
   if (key.dim() != 3 || value.sizes() != key.sizes() || value.scalar_type() != key.scalar_type())
     value_error("key and value must be (tokens, kv heads, head size) of one type");
@@ -299,6 +311,7 @@ PyObject* attend(PyObject* const* a) {
   Maybe out = maybe(a[9], "out");
   const int64_t window = integer(a[7]);
   const bool want = truth(a[10]);
+  no_gradient("kv_attend", {&q, &kv, get(scales), get(out)});
   if (q.dim() != 3) value_error("q must be (tokens, heads, head size)");
   const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
   const at::Device dev = q.device();

@@ -10,7 +10,8 @@ page bt[r, p // slots], slot p % slots.  Tokens past qsl[-1] are a captured step
 
 One launch appends (csrc/kv_append.hip) and one to three attend (csrc/kv_attend.hip), on the current stream, without
 waiting and without a read of the device on the host, so both can be captured in a graph.  Arguments are checked in
-csrc/bind.cpp.  There is no CPU implementation.
+csrc/bind.cpp.  Neither has a gradient: with grad mode on, tensors that require one are refused.  There is no CPU
+implementation.
 """
 from __future__ import annotations
 

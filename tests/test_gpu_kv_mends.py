@@ -9,7 +9,7 @@ import torch
 
 from oracle import paged
 from sdcguard_amd import _lib
-from tests.test_gpu_kv_attn import DEV, append_checked, attend_checked, make, step
+from tests.test_gpu_kv_attn import DEV, _turns, append_checked, attend_checked, make, step
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +210,29 @@ def test_queries_up_to_the_largest_number(large):
     c["q"][:, :, 5] = torch.finfo(torch.bfloat16).max
     c["q"][1::2, :, 5] *= -1.0
     attend_tight(tall(c) if large else c)
+
+
+def test_calls_that_would_drop_a_gradient_are_refused():
+    from sdcguard_amd.kv_attn import kv_append, kv_attend
+    from sdcguard_amd.rope import rotate
+    c = make(((20, 2), (5, 1)), seed=27, garbage=False)
+    k, v, q, kv, sc, st = c["k"], c["v"], c["q"], c["kv"], c["scales"], step(c)
+    turns, pos = _turns(64), torch.arange(3, device=DEV)
+    leaf = lambda t: t.clone().requires_grad_()                                                   # noqa: E731
+    calls = (lambda: kv_append(leaf(k), v, kv, sc, *st), lambda: kv_append(k, leaf(v), kv, sc, *st),
+             lambda: kv_append(k, v, kv, leaf(sc), *st), lambda: kv_append(k, v, kv, sc, *st, turns=leaf(turns)),
+             lambda: kv_append(k, v, kv, sc, *st, query=leaf(q)),
+             lambda: kv_append(k, v, kv, sc, *st, query=q, query_out=leaf(q)),
+             lambda: kv_attend(leaf(q), kv, sc, *st), lambda: kv_attend(q, kv, leaf(sc), *st),
+             lambda: kv_attend(q, kv, sc, *st, out=leaf(q)), lambda: rotate(q, pos, leaf(turns)))
+    codes, before = kv.view(torch.uint8).clone(), sc.clone()
+    for call in calls:
+        with pytest.raises(ValueError, match="takes? no gradient"):
+            call()
+    assert torch.equal(codes, kv.view(torch.uint8)) and torch.equal(before, sc)
+    with torch.no_grad():
+        for call in calls:
+            call()
+        assert torch.equal(kv_attend(leaf(q), kv, sc, *st), kv_attend(q, kv, sc, *st))
+    with torch.inference_mode():
+        kv_attend(q, kv, sc, *st)
