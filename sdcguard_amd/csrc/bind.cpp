@@ -68,7 +68,12 @@ bool truth(PyObject* o) {
 }
 
 // The cache's operators, and a rotation's frequencies, have no gradient: rather than drop one the call is refused.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t && t->_fw_grad(/*level=*/0).defined()) value_error(std::string(what) + ": no forward-mode gradient");
+}
 void no_gradient(const char* what, std::initializer_list<const Tensor*> ts) {
+  no_tangent(what, ts);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : ts)
     if (t && t->requires_grad())
@@ -179,6 +184,7 @@ PyObject* rotate(PyObject* const* a) {
   const Maybe out = maybe(a[6], "out");
   if (x.dim() < 3) value_error("x must be (..., tokens, heads, head size)");
   no_gradient("turns", {&turns});
+  no_tangent("rotate", {&x, get(out)});
   const at::Device dev = x.device();
   check_turns(turns, x.size(-1), dev);
   const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 2);

@@ -236,3 +236,24 @@ def test_calls_that_would_drop_a_gradient_are_refused():
         assert torch.equal(kv_attend(leaf(q), kv, sc, *st), kv_attend(q, kv, sc, *st))
     with torch.inference_mode():
         kv_attend(q, kv, sc, *st)
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+    from sdcguard_amd.kv_attn import kv_append, kv_attend
+    from sdcguard_amd.rope import rotate
+    c = make(((20, 2), (5, 1)), seed=28, garbage=False)
+    k, v, q, kv, sc, st = c["k"], c["v"], c["q"], c["kv"], c["scales"], step(c)
+    turns, pos = _turns(64), torch.arange(3, device=DEV)
+    codes = kv.view(torch.uint8).clone()
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))                              # noqa: E731
+        for call in (lambda: rotate(dual(q), pos, turns), lambda: rotate(q, pos, dual(turns)),
+                     lambda: rotate(q, pos, turns, out=dual(q.clone())),
+                     lambda: rotate(dual(q.float()).requires_grad_(), pos, turns),
+                     lambda: kv_append(dual(k), v, kv, sc, *st), lambda: kv_append(k, v, kv, sc, *st, query=dual(q)),
+                     lambda: kv_attend(dual(q), kv, sc, *st)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(ValueError, match="forward-mode"):
+                    call()
+    assert torch.equal(codes, kv.view(torch.uint8))
