@@ -80,6 +80,12 @@ void no_gradient(const char* what, std::initializer_list<const Tensor*> ts) {
       value_error(std::string(what) + " takes no gradient: detached tensors, or torch.no_grad(), are needed");
 }
 const Tensor* get(const Maybe& t) { return t ? &*t : nullptr; }
+// What a call has written to: autograd then knows of it where it kept the former values.  (Tensors of inference mode have no
+// version.)
+void written(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 
 int half_code(const Tensor& t) {
   if (t.scalar_type() == at::kBFloat16) return 0;
@@ -203,6 +209,7 @@ PyObject* rotate(PyObject* const* a) {
     const Tensor o3 = x.dim() > 3 ? out->view(x3.sizes()) : *out;
     const hipStream_t s = stream_of(x);
     check(unlocked([&] { return launch_rotation(x3, o3, pos, turns, how, s); }), "sdc_rope");
+    written({&*out});
     Py_INCREF(a[6]);
     return a[6];
   }
@@ -304,6 +311,7 @@ PyObject* append(PyObject* const* a) {
               Hq, s);
         }),
         "sdc_kv_append");
+  written({&kv, get(sc), made ? nullptr : get(out)});
   if (!query) Py_RETURN_NONE;
   if (made) return THPVariable_Wrap(*out);
   Py_INCREF(a[12]);
@@ -359,8 +367,12 @@ PyObject* attend(PyObject* const* a) {
         }),
         "sdc_kv_attend");
   PyObject* o = a[9];
-  if (made) o = THPVariable_Wrap(*out);
-  else Py_INCREF(o);
+  if (made) {
+    o = THPVariable_Wrap(*out);
+  } else {
+    written({&*out});
+    Py_INCREF(o);
+  }
   if (!want || !o) return o;
   PyObject* e = THPVariable_Wrap(lse);
   if (!e) {

@@ -257,3 +257,34 @@ def test_forward_mode_tangents_are_refused():
                 with mode(), pytest.raises(ValueError, match="forward-mode"):
                     call()
     assert torch.equal(codes, kv.view(torch.uint8))
+
+
+def test_autograd_knows_what_was_written_in_place():
+    from sdcguard_amd.kv_attn import kv_append, kv_attend, make_cache
+    from sdcguard_amd.rope import rotate
+    c = make(((20, 2), (5, 1)), seed=29, garbage=False)
+    k, v, q, kv, sc, st = c["k"], c["v"], c["q"].contiguous(), c["kv"], c["scales"], step(c)
+    turns, pos = _turns(64), torch.arange(3, device=DEV)
+    x = q.float().requires_grad_()
+    y = x * 2.0
+    z = (y * y).sum()                                  # y is kept for the gradient
+    with torch.no_grad():
+        rotate(y, pos, turns, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    full, _ = make_cache(4, 2, 16, 64, torch.bfloat16, DEV)
+    for call, wrote, kept in ((lambda: kv_append(k, v, kv, sc, *st), (kv, sc), (k, v)),
+                              (lambda: kv_append(k, v, kv, sc, *st, query=q), (kv, sc), (k, v, q)),
+                              (lambda: kv_append(k, v, kv, sc, *st, query=q, query_out=q), (kv, sc, q), (k, v)),
+                              (lambda: kv_append(k, v, full, None, *st), (full,), (k, v)),
+                              (lambda: kv_attend(q, kv, sc, *st, out=c["q"]), (c["q"],), (q, kv, sc)),
+                              (lambda: kv_attend(q, kv, sc, *st), (), (q, kv, sc)),
+                              (lambda: rotate(q, pos, turns), (), (q, pos, turns))):
+        before = [t._version for t in wrote + kept]
+        call()
+        after = [t._version for t in wrote + kept]
+        assert all(b > a for a, b in zip(before, after[:len(wrote)])) and after[len(wrote):] == before[len(wrote):]
+    with torch.inference_mode():
+        held, hs = make_cache(4, 2, 16, 64, device=DEV)
+        kv_append(k, v, held, hs, *st)
+    kv_append(k, v, held, hs, *st)                     # (tensors of inference mode have no version to raise)
