@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -85,6 +86,18 @@ const Tensor* get(const Maybe& t) { return t ? &*t : nullptr; }
 void written(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+// A tensor that is written: no element of it twice, and none of it also an input's unless it is that input (`same`) as a whole.
+void check_written(const char* name, const Tensor& t, const Tensor* same, std::initializer_list<const Tensor*> others) {
+  if (at::has_internal_overlap(t) == at::MemOverlap::Yes) value_error(std::string(name) + " must not hold an element twice");
+  if (same && at::get_overlap_status(t, *same) == at::MemOverlapStatus::Partial)
+    value_error(std::string(name) + " must be the input itself or share no memory with it");
+  for (const Tensor* o : others) {
+    const at::MemOverlapStatus s = at::get_overlap_status(t, *o);
+    if (s == at::MemOverlapStatus::Partial || s == at::MemOverlapStatus::Full)
+      value_error(std::string(name) + " must share no memory with the call's other tensors");
+  }
 }
 
 int half_code(const Tensor& t) {
@@ -206,6 +219,7 @@ PyObject* rotate(PyObject* const* a) {
     if (out->sizes() != x.sizes() || out->scalar_type() != x.scalar_type() || out->device() != dev)
       value_error("out must have x's shape, type and device");
     if (grad && (x.requires_grad() || out->requires_grad())) value_error("out takes no gradient: rotate without it");
+    check_written("out", *out, &x, {});
     const Tensor o3 = x.dim() > 3 ? out->view(x3.sizes()) : *out;
     const hipStream_t s = stream_of(x);
     check(unlocked([&] { return launch_rotation(x3, o3, pos, turns, how, s); }), "sdc_rope");
@@ -295,8 +309,12 @@ PyObject* append(PyObject* const* a) {
       made = true;
     } else if (out->sizes() != query->sizes() || out->scalar_type() != query->scalar_type() || out->device() != dev) {
       value_error("query_out must have query's shape, type and device");
+    } else {
+      check_written("query_out", *out, &*query, {&key, &value, &kv});
     }
   }
+  check_written("kv", kv, nullptr, {&key, &value});
+  if (code != SIXTEEN) check_written("scales", *scales, nullptr, {});
   const hipStream_t s = stream_of(key);
   const Maybe sc = code == SIXTEEN ? Maybe() : scales;
   check(unlocked([&] {
@@ -348,6 +366,8 @@ PyObject* attend(PyObject* const* a) {
     made = true;
   } else if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type() || out->device() != dev) {
     value_error("out must have q's shape, type and device");
+  } else {
+    check_written("out", *out, &q, {&kv});
   }
   Tensor lse, ws;
   if (want) lse = at::empty({T, Hq}, q.options().dtype(at::kFloat));

@@ -288,3 +288,27 @@ def test_autograd_knows_what_was_written_in_place():
         held, hs = make_cache(4, 2, 16, 64, device=DEV)
         kv_append(k, v, held, hs, *st)
     kv_append(k, v, held, hs, *st)                     # (tensors of inference mode have no version to raise)
+
+
+def test_outputs_that_overlap_are_refused():
+    from sdcguard_amd.kv_attn import kv_append, kv_attend
+    from sdcguard_amd.rope import rotate
+    c = make(((20, 2), (5, 1)), seed=30, garbage=False)
+    k, v, kv, sc, st = c["k"], c["v"], c["kv"], c["scales"], step(c)
+    q = c["q"].contiguous()
+    turns, pos = _turns(64), torch.arange(3, device=DEV)
+    long = torch.randn(4, 4, 64, device=DEV).bfloat16()
+    once = torch.empty(1, 4, 64, device=DEV, dtype=torch.bfloat16).expand(3, 4, 64)
+    flat = torch.randn(3 * 4 * 64, device=DEV).bfloat16()
+    kk = flat[:3 * 2 * 64].view(3, 2, 64)
+    for call in (lambda: rotate(long[1:], pos, turns, out=long[:3]), lambda: rotate(long[:3], pos, turns, out=once),
+                 lambda: kv_append(k, v, kv, sc, *st, query=long[1:], query_out=long[:3]),
+                 lambda: kv_append(k, v, kv, sc, *st, query=q, query_out=once),
+                 lambda: kv_append(kk, v, kv, sc, *st, query=q, query_out=flat.view(3, 4, 64)),
+                 lambda: kv_append(k, v, kv[:1].expand_as(kv), sc, *st),
+                 lambda: kv_append(k, v, kv, sc[:1].expand_as(sc), *st),
+                 lambda: kv_attend(long[1:], kv, sc, *st, out=long[:3]), lambda: kv_attend(q, kv, sc, *st, out=once)):
+        with pytest.raises(ValueError, match="memory|twice"):
+            call()
+    want = kv_attend(q, kv, sc, *st)
+    assert torch.equal(kv_attend(q, kv, sc, *st, out=q), want) and torch.equal(q, want)           # (in place)
