@@ -210,6 +210,8 @@ PyObject* rotate(PyObject* const* a) {
   Tensor pos = positions;
   if (pos.sizes() != lead && pos.dim() < (int64_t)lead.size() && pos.sizes() == lead.slice(lead.size() - pos.dim()))
     pos = pos.expand(lead);
+  else if (lead.size() > 1 && pos.dim() > 1 && pos.sizes() != lead)
+    value_error("positions are of the leading dimensions' shape, of the last of them, or one row for all tokens");
   const Tensor x3 = x.dim() > 3 ? x.flatten(0, -3) : x;
   pos = check_positions(pos, x3.size(0), dev);
   if (x.scalar_type() != at::kFloat) half_code(x);

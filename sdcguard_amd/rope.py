@@ -71,8 +71,8 @@ def frequencies(rot: int, base: float = 10000.0, scaling: Optional[dict] = None,
 
 def rotate(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, interleaved: bool = False,
            mscale: float = 1.0, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x (tokens, heads, head size), or with more leading dimensions, rotated by `positions` (one per token; a tensor of
-    the leading dimensions' shape, or of the last of them).  bf16, fp16 or fp32, any strides.  Differentiable in x; with
+    """x (tokens, heads, head size), or with more leading dimensions, rotated by `positions` (one per token: a tensor of
+    the leading dimensions' shape, of the last of them, or one row for all tokens in their order).  bf16, fp16 or fp32, any strides.  Differentiable in x; with
     `out` (x itself to rotate in place) it writes there and takes no gradient.  `inverse` rotates by the negative
     angles.  Queued on the current stream of x's device."""
     return _lib.bound().rotate(x, positions, turns, interleaved, mscale, inverse, out)

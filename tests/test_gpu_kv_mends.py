@@ -312,3 +312,16 @@ def test_outputs_that_overlap_are_refused():
             call()
     want = kv_attend(q, kv, sc, *st)
     assert torch.equal(kv_attend(q, kv, sc, *st, out=q), want) and torch.equal(q, want)           # (in place)
+
+
+def test_positions_of_another_shape_are_refused():
+    """As many positions as tokens, but not the tokens' shape: they would go to the wrong ones."""
+    from sdcguard_amd.rope import rotate
+    x, turns = torch.randn(6, 5, 4, 64, device=DEV), _turns(64)
+    pos = torch.randint(0, 9000, (6, 5), device=DEV)
+    want = rotate(x, pos, turns)
+    assert torch.equal(rotate(x, pos.reshape(-1), turns), want)
+    for bad in (pos.t().contiguous(), pos.t(), pos.view(3, 10), pos.view(1, 30), pos.view(6, 5, 1), pos[:, :1], pos[:1]):
+        with pytest.raises(ValueError, match="positions"):
+            rotate(x, bad, turns)
+    assert torch.equal(rotate(x[0], pos[:1], turns), rotate(x[0], pos[0], turns))
