@@ -456,6 +456,7 @@ int sdc_rope(int dtype, const void* x, int64_t sxt, int64_t sxh, int64_t sxd, vo
  *   A page's scale: the smallest power of two that holds the largest finite |x| appended since its slot 0 was last
  *     written; where it grows, the page's other slots are rescaled to it.  Requests must not share pages they write.
  *   turns (rot/2), interleaved, mscale: as sdc_rope (rot 0: no rotation); positions (T) or NULL (the tokens' own).
+ *   R may be 0, and W: seq_lens and bt, which then hold nothing, may be NULL.
  *   q (T, Hq, D), or NULL: rotated into q_out (which may be q); rows past qsl[R] become zeros. */
 int sdc_kv_append(int dtype, int cache, const void* key, int64_t skt, int64_t skh, int64_t skd, const void* val,
                   int64_t svt, int64_t svh, int64_t svd, int64_t T, int64_t Hkv, int64_t D, void* kv, int64_t cb,

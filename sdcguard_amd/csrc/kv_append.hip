@@ -518,7 +518,7 @@ extern "C" int sdc_kv_append(int dtype, int cache, const void* key, int64_t skt,
       (positions && pos_bytes != 4 && pos_bytes != 8) || (q && (Hq < 1 || !q_out)))
     return SDC_EINVAL;
   if (T == 0) return SDC_OK;
-  if (!key || !val || !kv || !qsl || !seq_lens || !bt || (rot && !turns) || (cache != SDC_CACHE_16 && !scales))
+  if (!key || !val || !kv || !qsl || (R && !seq_lens) || (R && W && !bt) || (rot && !turns) || (cache != SDC_CACHE_16 && !scales))
     return SDC_EINVAL;
   if (T > 0x3FFFFFFF || R > 0x0FFFFFFF || Hkv * D > 1 << 24 || (q && Hq * D > 1 << 24)) return SDC_EUNSUPPORTED;
   const int64_t es = cache == SDC_CACHE_16 ? 2 : 1;

@@ -1502,7 +1502,7 @@ extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, i
       max_len < 0 || max_len > W * N)
     return SDC_EINVAL;
   if (T == 0) return SDC_OK;
-  if (!q || !o || !kv || !scales || !qsl || !seq_lens || !bt) return SDC_EINVAL;
+  if (!q || !o || !kv || !scales || !qsl || (R && !seq_lens) || (R && W && !bt)) return SDC_EINVAL;
   if (T > 0x3FFFFFFF || R > 0x0FFFFFFF || Hq > 65536 || W * N > 0x7FFFFFFF || max_len > 0x3FFFFFFF)
     return SDC_EUNSUPPORTED;                    // (numbers of keys are added up in 32 bits)
   AttendArgs a{};

@@ -325,3 +325,22 @@ def test_positions_of_another_shape_are_refused():
         with pytest.raises(ValueError, match="positions"):
             rotate(x, bad, turns)
     assert torch.equal(rotate(x[0], pos[:1], turns), rotate(x[0], pos[0], turns))
+
+
+@pytest.mark.parametrize("T", [1, 40, 3000])
+def test_steps_without_requests_and_tables_without_pages(T):
+    """A captured step that is all padding, and requests that have no page: nothing is written, zeros and -inf come out."""
+    from sdcguard_amd.kv_attn import kv_append, kv_attend
+    for D in (64, 40):
+        for R, W in ((0, 5), (0, 0), (2, 0), (0, 200000)):
+            c = make(((20, 2),), D=D, Hq=8, Hkv=2, seed=31, garbage=False)
+            k, v = (torch.randn(T, 2, D, device=DEV).bfloat16() for _ in range(2))
+            q = torch.randn(T, 8, D, device=DEV).bfloat16()
+            st = (torch.full((R + 1,), min(R, 1) * T, device=DEV, dtype=torch.int32),
+                  torch.full((R,), T, device=DEV, dtype=torch.int32), torch.zeros(R, W, device=DEV, dtype=torch.int32))
+            st[0][0] = 0
+            codes, sc = c["kv"].view(torch.uint8).clone(), c["scales"].clone()
+            rotated = kv_append(k, v, c["kv"], c["scales"], *st, turns=_turns(D), query=q)
+            o, lse = kv_attend(q, c["kv"], c["scales"], *st, return_lse=True)
+            assert not o.any() and torch.isneginf(lse).all() and bool(rotated.any()) == (R > 0)
+            assert torch.equal(codes, c["kv"].view(torch.uint8)) and torch.equal(sc, c["scales"])
