@@ -356,6 +356,8 @@ PyObject* attend(PyObject* const* a) {
     value_error(std::to_string(Hq) + " heads of " + std::to_string(D) + " over " + std::to_string(Hkv) +
                 " kv heads: a multiple of them, and head sizes up to 256");
   if (window < 0) value_error("window must not be negative (0: none)");
+  const float scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)number(a[6]);
+  if (!std::isfinite(scale)) value_error("scale must be a finite number");
   const Step st = step(a[3], a[4], a[5], dev);
   const int64_t R = st.lens.size(0), W = st.bt.size(1);
   int64_t most = W * N;
@@ -376,7 +378,6 @@ PyObject* attend(PyObject* const* a) {
   // (a workspace of the call's own: the allocator orders its memory by stream, and within a captured graph keeps it)
   const int64_t need = g_entry.workspace(T, R, Hq, Hkv, D, N, most, window);
   if (need) ws = at::empty({need}, q.options().dtype(at::kByte));
-  const float scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)number(a[6]);
   const hipStream_t s = stream_of(q);
   check(unlocked([&] {
           return g_entry.attend(dt, code, q.const_data_ptr(), q.stride(0), q.stride(1), q.stride(2), out->data_ptr(),

@@ -9,6 +9,7 @@
 // any head size and alignment, a row a wave; parts whose value scales are far from 1 are left to the same (plain_row).
 // A part of a tile's keys is one workgroup's; kv_attend_join joins the parts in their order.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -1499,7 +1500,7 @@ extern "C" int sdc_kv_attend(int dtype, int cache, const void* q, int64_t sqt, i
   SDC_CLEAR_ERRORS();
   if ((dtype != SDC_BF16 && dtype != SDC_FP16) || (cache != SDC_CACHE_E4M3 && cache != SDC_CACHE_I8) || T < 0 ||
       Hq < 1 || Hkv < 1 || Hq % Hkv || D < 1 || D > ANY_D || NB < 1 || N < 1 || N > 65536 || R < 0 || W < 0 || window < 0 ||
-      max_len < 0 || max_len > W * N)
+      max_len < 0 || max_len > W * N || !std::isfinite(scale))
     return SDC_EINVAL;
   if (T == 0) return SDC_OK;
   if (!q || !o || !kv || !scales || !qsl || (R && !seq_lens) || (R && W && !bt)) return SDC_EINVAL;

@@ -344,3 +344,11 @@ def test_steps_without_requests_and_tables_without_pages(T):
             o, lse = kv_attend(q, c["kv"], c["scales"], *st, return_lse=True)
             assert not o.any() and torch.isneginf(lse).all() and bool(rotated.any()) == (R > 0)
             assert torch.equal(codes, c["kv"].view(torch.uint8)) and torch.equal(sc, c["scales"])
+
+
+def test_scales_that_are_no_numbers_are_refused():
+    from sdcguard_amd.kv_attn import kv_attend
+    c = make(((20, 2), (5, 1)), seed=32)
+    for scale in (float("nan"), float("inf"), -1e300):
+        with pytest.raises(ValueError, match="finite"):
+            kv_attend(c["q"], c["kv"], c["scales"], *step(c), scale=scale)

@@ -106,3 +106,8 @@ def test_a_window_wider_than_any_length_is_none(window):
     for T, R, N, most in ((1, 1, 16, 200000), (1, 1, 1, 5000), (64, 64, 16, 131072), (4096, 2, 16, 131072), (3, 0, 8, 70000)):
         assert need(T, R, 32, 8, 128, N, most, window) == need(T, R, 32, 8, 128, N, most, 0)
     assert need(1, 1, 32, 8, 128, 16, 200000, window) > 0
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_attention_refuses_scales_that_are_no_numbers(scale):
+    assert _attend(scale=scale) == _lib.SDC_EINVAL
