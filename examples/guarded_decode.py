@@ -4,9 +4,9 @@
 
 The queries and keys of a layer are rotated by position with their gradient (rope.rotate) for a few training steps.  The
 trained layer then serves two sequences: their prompts as chunks, the rest token by token.  Each step verifies the pages
-that earlier steps wrote (KVLedger), appends its keys and values, rotated and quantized on the way (kv_attn.kv_append),
-attends over the cache (kv_attn.kv_attend) and records the pages it changed.  At the end the outputs are compared with the
-layer's 16-bit attention, and one flipped bit of the cache has to be found.
+that earlier steps wrote, codes and scales (a KVLedger each), appends its keys and values, rotated and quantized on the way
+(kv_attn.kv_append), attends over the cache (kv_attn.kv_attend) and records the pages it changed.  At the end the outputs are
+compared with the layer's 16-bit attention, and one flipped bit of the codes and one of the scales have to be found.
 """
 from __future__ import annotations
 
@@ -66,13 +66,14 @@ def train(layer, x, steps=3, rate=0.05):
 
 
 def serve(layer, xs, prompt, cache):
-    """The sequences' outputs, served over a paged cache: (outputs, cache, scales, table, ledger, mismatched pages)."""
+    """The sequences' outputs, served over a paged cache: (outputs, cache, scales, table, ledgers, mismatched pages)."""
     dev, R, n = xs[0].device, len(xs), xs[0].shape[0]
     width = -(-n // SLOTS)
     kv, scales = make_cache(R * width + 1, KV_HEADS, SLOTS, DIM, CACHES[cache], dev)
     order = torch.randperm(R * width, generator=torch.Generator().manual_seed(2)).to(torch.int32)
     table = (order + 1).view(R, width).to(dev)                   # page 0 stays empty
-    ledger = KVLedger(kv.view(torch.uint8), R, width)
+    # (a scale multiplies a whole page of a head: unguarded, one flipped bit of it would go unseen)
+    ledgers = KVLedger(kv.view(torch.uint8), R, width), KVLedger(scales, R, width)
     outs, bad, at = [[] for _ in xs], 0, 0
     column = torch.arange(width, device=dev)
     with torch.no_grad():
@@ -81,16 +82,17 @@ def serve(layer, xs, prompt, cache):
             x = torch.cat([s[at:at + new] for s in xs])
             qsl = torch.arange(R + 1, device=dev, dtype=torch.int32) * new
             lens = torch.full((R,), at + new, device=dev, dtype=torch.int32)
-            bad += int(ledger.verify(table).count)
+            bad += sum(int(ledger.verify(table).count) for ledger in ledgers)
             q, k, v = layer.project(x)
             q = kv_append(k, v, kv, scales, qsl, lens, table, turns=layer.turns, mscale=layer.mscale, query=q)
             o = kv_attend(q, kv, scales, qsl, lens, table, max_seq_len=n)
             written = (column >= at // SLOTS) & (column <= (at + new - 1) // SLOTS)
-            ledger.record(table, written.expand(R, width))
+            for ledger in ledgers:
+                ledger.record(table, written.expand(R, width))
             for r in range(R):
                 outs[r].append(o[r * new:(r + 1) * new])
             at += new
-    return [torch.cat(o) for o in outs], kv, scales, table, ledger, bad
+    return [torch.cat(o) for o in outs], kv, scales, table, ledgers, bad
 
 
 def main(tokens=48, cache="e4m3", quiet=False):
@@ -100,15 +102,17 @@ def main(tokens=48, cache="e4m3", quiet=False):
     g = torch.Generator(device=dev).manual_seed(3)
     xs = [torch.randn(tokens, HEADS * DIM, generator=g, device=dev) for _ in range(2)]
     losses = train(layer, xs[0])
-    outs, kv, scales, table, ledger, bad = serve(layer, xs, max(1, tokens // 2), cache)
+    outs, kv, scales, table, (codes_ledger, scales_ledger), bad = serve(layer, xs, max(1, tokens // 2), cache)
     with torch.no_grad():
         wants = [layer.attend(x) for x in xs]
     off = max(float((o.float() - w).abs().max() / w.abs().max()) for o, w in zip(outs, wants))
-    kv.view(torch.uint8)[table[1, 0].long(), 0, 3, 5] ^= 4        # one flipped bit
-    found = ledger.verify(table).read()
+    kv.view(torch.uint8)[table[1, 0].long(), 0, 3, 5] ^= 4        # one flipped bit of a code, one of a scale's exponent
+    scales.view(torch.int32)[table[0, 0].long(), 1, 0] ^= 1 << 24
+    found = codes_ledger.verify(table).read()
+    found["scale_entries"] = scales_ledger.verify(table).read()["entries"]
     if not quiet:
         print(f"loss {' -> '.join(f'{x:.4f}' for x in losses)}; {tokens} tokens over a {cache} cache: off by {off:.3f} of the "
-              f"largest output; pages changed unseen: {bad}; after a flipped bit: {found['entries']}")
+              f"largest output; pages changed unseen: {bad}; after a flipped bit of the codes: {found['entries']}, of the scales: {found['scale_entries']}")
     return losses, off, bad, found
 
 

@@ -2,6 +2,7 @@
 scales at both ends of their types, steps and tables of nothing, and what autograd has to know of their calls."""
 from __future__ import annotations
 
+import importlib.util
 import math
 
 import pytest
@@ -352,3 +353,13 @@ def test_scales_that_are_no_numbers_are_refused():
     for scale in (float("nan"), float("inf"), -1e300):
         with pytest.raises(ValueError, match="finite"):
             kv_attend(c["q"], c["kv"], c["scales"], *step(c), scale=scale)
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "int8"])
+def test_the_example_guards_the_scales_too(cache):
+    from tests.test_gpu_guarded_decode import PATH
+    spec = importlib.util.spec_from_file_location("guarded_decode", PATH)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    _, _, bad, found = m.main(48, cache, quiet=True)
+    assert bad == 0 and found["entries"] == [(1, 0)] and found["scale_entries"] == [(0, 0)]
