@@ -242,9 +242,9 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int item, int h
   const int units = n * nu;
 
   // Up to HELD units a lane stay in registers, all loads of keys and values on their way at once (a token of 64 sequences each:
-  // 6.6 us, 12 with the two passes below, which larger pages take).
+  // 6.4 us, 12 with the two passes below, which larger pages take).
   constexpr int HELD = 2;
-  if (units <= step * HELD && n * P <= HOLD) {
+  if (SHARE == 1 || (units <= step * HELD && n * P <= HOLD)) {           // (a wave alone: always, by launch()'s choice)
     float x[HELD][2 * UP], y[HELD][2 * UP];
     RopeUnit ru[HELD], rv[HELD];
     int tok[HELD];
@@ -463,8 +463,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 }
 template <int DT, int CT, int UP>
 int launch(AppendArgs a, hipStream_t stream) {
-  // four waves share a head where a page holds more units than one keeps in registers (64 slots of 128: 200 tokens in
-  // four chunks 24 us, 33 with a wave a head); a workgroup takes up to 1024 units of queries
+  // four waves share a head where a page holds more units than one keeps in registers (chunks of 50 tokens into pages of 64
+  // slots of 128: 10 us, 33 with a wave a head); a workgroup takes up to 1024 units of queries
   const int nu = sdc_units(a.D, UP);
   const bool share = a.st.N * nu > 128;
   a.hgroups = share ? a.Hkv : (int)sdc_cdiv(a.Hkv, 4);
