@@ -211,18 +211,23 @@ __device__ __forceinline__ u16x2 wave_larger(u16x2 v) {
 }
 // How a page's value scale enters the products: as 2^b times a factor in [1/2, 1).  2^(x + b), x a score, is what a probability's
 // product with its scale is rounded in, so it is that exponent whose maximum is followed; the sum of probabilities takes 2^-b of
-// it.  With b from LOW_B to HIGH_B neither loses keys to fp32's ends.  Zero, and the scale 2^-126 of a page of zeros, count as
-// 2^LOW_B, with their values next to nothing.
+// it.  With b from LOW_B to HIGH_B neither loses keys to fp32's ends.  A part with scales outside that (values of 1e15 and more,
+// or under 4e-16) takes them all relative to a 2^ve; zero, and the scale 2^-126 of a page of zeros, count as LOW_B then too.
 constexpr int LOW_B = -60, HIGH_B = 40;
-__device__ __forceinline__ int scale_exponent(float v) {
+__device__ __forceinline__ int scale_exponent(float v, int ve) {
   const int f = (int)scale_field(v);
-  return f > 1 ? f - 126 : fabsf(v) < 1.f ? LOW_B : 0;
+  return f ? max(f - 126 - ve, LOW_B) : v == 0.f ? LOW_B : 0;
 }
 __device__ __forceinline__ float scale_factor(float v, int b) { return ldexpf(v, -b); }
-// Whether a part has scales outside that (values of 1e15 and more, or under 4e-16): it is left to plain_row.
-__device__ __forceinline__ bool scales_far(u16x2 ends) {
+// From the ends of a part's scales: whether no ve is right (values as 1e15 beside 1e-15), and it is left to plain_row; and ve, 0
+// but for such parts as above.
+__device__ __forceinline__ bool scales_apart(u16x2 ends) {
   const int top = __builtin_amdgcn_readfirstlane(ends.x), low = __builtin_amdgcn_readfirstlane(ends.y);
-  return top > 126 + HIGH_B || top == 1 || (low && 255 - low < 126 + LOW_B);
+  return low && top - (255 - low) > HIGH_B - LOW_B;
+}
+__device__ __forceinline__ int scale_unit(u16x2 ends) {
+  const int top = __builtin_amdgcn_readfirstlane(ends.x), low = __builtin_amdgcn_readfirstlane(ends.y);
+  return top <= 126 + HIGH_B && top != 1 && (!low || 255 - low >= 126 + LOW_B) ? 0 : top - 126 - HIGH_B;
 }
 
 // Over the lanes l, l + 16, l + 32, l + 48: rows of 16 swapped by VALU moves (a trip through LDS takes ten times as long;
@@ -513,7 +518,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) voi
     float2 sc = sc0;
     if (i != tid) sc = {scp[0], scp[1]};
     if (page < 0) sc = {__builtin_nanf(""), __builtin_nanf("")};
-    const int b = scale_exponent(sc.y);
+    const int b = scale_exponent(sc.y, 0);
     sh.h.ks[i] = {sc.x, (float)b};
     sh.h.vs[i] = {ldexpf(1.f, -b), scale_factor(sc.y, b)};
     ends = scale_ends(ends, sc.y);
@@ -553,10 +558,20 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) voi
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NW; ++i) ends = __builtin_elementwise_max(ends, wends[i]);
-  if (scales_far(ends)) {
+  if (scales_apart(ends)) {
     __syncthreads();                           // (the tables' place is the plain rows')
     plain_part<CT>(&sh.plain[0][0], NW);
-    return;
+    __builtin_amdgcn_endpgm();                 // (after a return in its place the rest spills 60 scalar registers)
+  }
+  const int ve = scale_unit(ends);
+  if (ve != 0) {
+    for (int i = tid; i < np; i += 64 * NW) {
+      const float v = ldexpf(sh.h.vs[i].y, (int)sh.h.ks[i].y);
+      const int b = scale_exponent(v, ve);
+      sh.h.ks[i].y = (float)b;
+      sh.h.vs[i] = {ldexpf(1.f, -b), scale_factor(v, b + ve)};
+    }
+    __syncthreads();
   }
   f16x8 qf[NS];
 #pragma unroll
@@ -732,11 +747,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) voi
       x += f * *reinterpret_cast<const f32x4*>(&sh.o[u][row][d]);
     }
     if (t.nsp == 1) {
-      write_row(a, t, tok, token, head, d, mt, 0.f, lt, x, BIAS);
+      write_row(a, t, tok, token, head, d, mt, (float)ve, lt, x, BIAS);
     } else {
       float* rec = sp.part + (int64_t)blockIdx.x * ROWS * (D + HEAD);
       constexpr float unit = 0x1p-13f;         // 2^-BIAS
-      if (d == 0) *reinterpret_cast<f32x4*>(rec + HEAD * row) = f32x4{mt, mt, lt * unit, 0.f};
+      if (d == 0) *reinterpret_cast<f32x4*>(rec + HEAD * row) = f32x4{mt + (float)ve, mt, lt * unit, 0.f};
       *reinterpret_cast<f32x4*>(rec + HEAD * ROWS + row * D + d) = x * unit;
     }
   }
@@ -797,7 +812,7 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   __shared__ Stage st[2];
   __shared__ WaveScales wscales[NW];
   __shared__ int32_t pg[MAXP];
-  __shared__ float4 ps[MAXP];                  // of each page: |ks|, log2 vs, 1 / vs, the factor on the stored values
+  __shared__ float4 ps[MAXP];                  // of each page (page_scales)
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int D = a.D, N = a.st.N;
@@ -834,6 +849,15 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
   const int64_t a0 = t.c0 + (int64_t)s * t.C, a1 = min(t.khi, a0 + t.C);
   const int64_t fp = (uint32_t)a0 / (uint32_t)N;
   const int np = (int)((uint32_t)(a1 - 1) / (uint32_t)N - fp) + 1, base0 = (int)(a0 - fp * N);
+  // |ks|; log2 of |vs| / 2^ve, at least LOW_B; the power of two that goes back; the factor on the stored values
+  auto page_scales = [](float ks, float vs, int ve) -> float4 {
+    const int f = (int)scale_field(vs);
+    const float v = ldexpf(fabsf(vs), -ve);
+    const bool log = f && f - 126 - ve >= LOW_B, small = !log && (f || vs == 0.f);
+    const float inv = log ? 1.f / v : small ? ldexpf(1.f, -LOW_B) : 1.f;
+    if (ks != ks) return {0.f, 0.f, ks, ks};
+    return {fabsf(ks), log ? log2f(v) : small ? (float)LOW_B : 0.f, inv, log ? (vs < 0.f ? -1.f : 1.f) : ldexpf(vs, -ve) * inv};
+  };
   // the queries: fragments of the lane's row, in fp16 after a power of two
   f16x8 qf[NS];
   float rf;
@@ -867,15 +891,12 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
       const int32_t p = a.st.bt[t.r * a.st.sbt + fp + i];
       const bool in = p >= 0 && p < a.st.NB;
       const float* scp = a.scales + (in ? (int64_t)p : 0) * a.sb + t.hk * a.sh;
-      const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf(""), v = fabsf(vs);
-      const bool log = scale_field(v) > 1, small = v < 0x1p-125f, key = ks == ks;
-      const float inv = log ? 1.f / v : small ? ldexpf(1.f, -LOW_B) : 1.f;
-      ps[i] = {key ? fabsf(ks) : 0.f, log ? log2f(v) : small ? (float)LOW_B : 0.f, !key ? ks : inv,
-               !key ? ks : log ? (vs < 0.f ? -1.f : 1.f) : vs * inv};
+      const float ks = in ? scp[0] : __builtin_nanf(""), vs = in ? scp[1] : __builtin_nanf("");
+      ps[i] = page_scales(ks, vs, 0);
       pg[i] = (in ? p : 0) | (ks < 0.f ? (int32_t)0x80000000 : 0);        // the sign of ks, which the keys take
       ends = scale_ends(ends, vs);
       flip |= ks < 0.f;
-      mul |= !log || vs < 0.f || !key;
+      mul |= ps[i].w != 1.f;
     }
     auto narrow = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
@@ -915,9 +936,18 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     mul |= x.mul;
   }
   const bool flips = __builtin_amdgcn_readfirstlane(flip), muls = __builtin_amdgcn_readfirstlane(mul);
-  if (scales_far(ends)) {
+  if (scales_apart(ends)) {
     plain_part<CT>(reinterpret_cast<float*>(st), NW);
-    return;
+    __builtin_amdgcn_endpgm();
+  }
+  const int ve = scale_unit(ends);
+  if (ve != 0) {
+    for (int i = tid; i < np; i += 2 * HT)
+      if (ps[i].z == ps[i].z) {                // (pages outside the cache, and whose key scale is NaN, are as they were)
+        const float* scp = a.scales + (int64_t)(pg[i] & 0x7FFFFFFF) * a.sb + t.hk * a.sh;
+        ps[i] = page_scales(scp[0], scp[1], ve);
+      }
+    __syncthreads();
   }
   // keys, counted from a0: those of the tile; those that the lane's row sees; those that a row of the wave, and every row of
   // the wave sees; those that every row of the tile sees
@@ -1279,12 +1309,12 @@ __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_at
     // (a row with keys whose scores are all -inf: 0 / 0)
     const int64_t p = t.p0 + r.tok;
     const bool any = min(p + 1, a.maxlen) > max(p - a.window + 1, (int64_t)0);
-    const float f = any ? 1.f / l : 0.f;
-    each([&](int d, f32x4 x) { write_four(a, r.token, r.head, d, x, f); });
+    const float half = ve == 0 ? 1.f : __builtin_amdgcn_exp2f(0.5f * (float)ve), f = any ? half / l : 0.f;
+    each([&](int d, f32x4 x) { write_four(a, r.token, r.head, d, x * f, half); });
     if (a.lse && h == 0) a.lse[r.token * a.slt + r.head] = any ? (m + log2f(l) - BIAS) * LN2 : NEG_INF;
   } else {
     float* rec = sp.part + ((int64_t)tile * sp.S + s) * TALL * (D + HEAD);
-    if (h == 0) *reinterpret_cast<f32x4*>(rec + HEAD * r.row) = f32x4{m, m, l * 0x1p-13f, 0.f};
+    if (h == 0) *reinterpret_cast<f32x4*>(rec + HEAD * r.row) = f32x4{m + (float)ve, m, l * 0x1p-13f, 0.f};
     each([&](int d, f32x4 x) { *reinterpret_cast<f32x4*>(rec + HEAD * TALL + r.row * D + d) = x * 0x1p-13f; });
   }
 }

@@ -363,3 +363,19 @@ def test_the_example_guards_the_scales_too(cache):
     spec.loader.exec_module(m)
     _, _, bad, found = m.main(48, cache, quiet=True)
     assert bad == 0 and found["entries"] == [(1, 0)] and found["scale_entries"] == [(0, 0)]
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("N", [16, 6])
+def test_value_scales_on_both_sides_of_each_limit(N, large):
+    """Pages of two scales, within what a part takes as they are, within what it takes relative to one, and past both; beside
+    pages of scale 0, of zeros, and of a subnormal scale."""
+    c = make(((300, 200), (90, 1), (1, 1)), D=64, Hq=4, Hkv=1, N=N, seed=33, garbage=False)
+    c = tall(c) if large else c
+    for hi, lo in ((39, -60), (40, -61), (41, -60), (42, -59), (80, -19), (80, -20), (80, -21), (-60, -70), (-61, -125), (-100, -126),
+                   (-125, -126), (-126, -126), (118, 19), (118, 17), (60, -60)):
+        for other in (2.0 ** lo, 0.0, 2.0 ** -126, 2.0 ** -135):
+            c["scales"][:, :, 1] = 2.0 ** hi
+            c["scales"][::3, :, 1] = 2.0 ** lo
+            c["scales"][::7, :, 1] = other
+            attend_tight(c)
