@@ -472,6 +472,7 @@ int sdc_kv_append(int dtype, int cache, const void* key, int64_t skt, int64_t sk
  *   dtype 0 = bf16, 1 = fp16 (q and o); cache 0 = e4m3, 1 = int8; kv, scales, qsl, seq_lens, bt as sdc_kv_append.
  *   max_len: no sequence is longer (keys past it are not read); at most W * N.  D <= 256, Hq a multiple of Hkv.
  *   A query without keys, and rows past qsl[R]: zeros and -inf.  A key whose page lies outside the cache is NaN.
+ *   scale: finite.  R and W as sdc_kv_append.  o may be q.
  *   workspace: sdc_kv_attend_workspace(T, R, Hq, Hkv, D, N, max_len, window) bytes (may be NULL where that is 0). */
 int64_t sdc_kv_attend_workspace(int64_t T, int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int64_t N, int64_t max_len,
                                 int64_t window);

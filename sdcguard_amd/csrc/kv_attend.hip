@@ -230,8 +230,8 @@ __device__ __forceinline__ int scale_unit(u16x2 ends) {
   return top <= 126 + HIGH_B && top != 1 && (!low || 255 - low >= 126 + LOW_B) ? 0 : top - 126 - HIGH_B;
 }
 
-// Over the lanes l, l + 16, l + 32, l + 48: rows of 16 swapped by VALU moves (a trip through LDS takes ten times as long;
-// 24 sequences with a chunk of 500 24.3 us, 26.1 so).
+// Over the lanes l, l + 16, l + 32, l + 48: rows of 16 swapped by VALU moves (a trip through LDS takes ten times as long:
+// 7 % of 24 sequences with a chunk of 500).
 template <class F>
 __device__ __forceinline__ float over_groups(float v, F join) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -371,7 +371,8 @@ __device__ __forceinline__ void plain_part(float* q, int waves) {
 // fp16; queries are scaled to it by a power of two per row (a bf16 element 2^-27 of its row's largest keeps all bits).
 // The key scales multiply the scores, the value scales the probabilities, in fp32.  Probabilities are rounded to fp16's
 // 11 bits, in units that put their largest product with a value scale at 2^12 .. 2^15 (scale_exponent).
-// Four sequences of 100-131k tokens, 8 heads of 128: 173 us, 5.6 TB/s; 64 of 512-2048 tokens 37 us; one of 500 11 us.
+// With fp16 outputs that leaves 1.4 times the error of fp32 probabilities against 64 bits; under bf16's own rounding it is gone.
+// Four sequences of 100-131k tokens, 8 heads of 128: 172 us, 5.6 TB/s; 64 of 512-2048 tokens 37 us; one of 500 11 us.
 template <int CT, int DP, int PN>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) void kv_attend_rows(AttendArgs a, Split sp) {
   constexpr int NW = 4, KEYS = 32 * NW;                     // keys that the workgroup's waves take at a time
@@ -785,8 +786,8 @@ __device__ __forceinline__ float over_halves_sum(float v) {
 // factors on the widened values; keys that a row does not see score -inf; values of NaN under a tile that some row sees only
 // in part are left out and put in at the end.  Rounding of the probabilities, and scales far from 1: as kv_attend_rows.
 //
-// Two chunks of 2048 tokens behind up to 3000 keys, 32 heads of 128: 285 us, 890 TFLOP/s; the matrix cores are busy 38 % of
-// it, LDS 27 %.  Waves of 32 rows: 64 would need all 512 registers, 16 twice the fragments.
+// Two chunks of 2048 tokens behind up to 3000 keys, 32 heads of 128: 293 us, 864 TFLOP/s; the matrix cores are busy 38 % of
+// it.  Waves of 32 rows: 64 would need all 512 registers, 16 twice the fragments.
 template <int CT, int DP, int PN>
 __global__ __launch_bounds__(64 * tall_waves(DP), tall_waves(DP) / 4) void kv_attend_tiles(AttendArgs a, Split sp) {
   constexpr int KT = DP > 128 ? 32 : 64, KB = KT / 32;                  // keys of a tile, blocks of 32
@@ -1395,7 +1396,7 @@ struct Plan {
 };
 constexpr int64_t CROSS = 640000000;           // small tiles x their keys x head size from which large ones are faster
 // Beside chunks, kv_attend_rows takes requests of up to so many of its tiles: with 1 / 2 / 4, 32 sequences of 6 tokens behind
-// 16k keys 522 / 268 / 271 us, 64 of 16 tokens behind 8k 474 / 481 / 424, 32 decoding beside a chunk of 2048 122 / 130 / 149.
+// 16k keys 518 / 270 / 272 us, 64 of 16 tokens behind 8k 460 / 460 / 424, 32 decoding beside a chunk of 2048 205 / 215 / 261.
 constexpr int FEW = 2;
 Split split_of(int rows, int64_t G, int64_t N) {
   Split sp{};
@@ -1428,14 +1429,14 @@ Plan plan(int64_t T, int64_t R, int64_t Hkv, int64_t G, int64_t D, int64_t N, in
   auto keys = [&](const Split& sp) { return std::min(max_len, seen(window) + sp.TB); };
   p.rows = split_of(ROWS, G, N);
   p.tiles = split_of(32 * tall_waves(D), G, N);
-  // One round of the workgroups that a lane's registers leave room for, two a CU: 64 sequences of 512-2048 tokens 34.5 us,
-  // four of 100-131k 179 us, 32 of 1000-4000 with their append 44 us (three rounds: 34.5, 184 and 45).  Parts of fewer than 512
-  // keys cost more to join than they save.  (Workgroups of eight waves, one a CU: 41, 182 and 42.)
+  // One round of the workgroups that a lane's registers leave room for, two a CU: 64 sequences of 512-2048 tokens 39 us,
+  // four of 100-131k 181 us, 32 of 1000-4000 with their append 51 us (three rounds: 48, 192 and 56).  Parts of fewer than 512
+  // keys cost more to join than they save.
   constexpr int64_t resident = 512;
   // More tokens than requests: some have a chunk.  The tiles of 16 rows read every key anew, those of 256 cost two more
-  // launches and fill the chip later: chunks behind 4096 keys, 32 heads, 127 / 505 / 1009 / 2017 tokens in small and in large
-  // tiles, heads of 128: 52 and 57 / 97 and 107 / 172 and 141 / 290 and 188 us, heads of 64: 33 and 42 / 58 and 76 / 96 and
-  // 99 / 157 and 132 us.
+  // launches and fill the chip later: a chunk behind 4096 keys, 32 heads, 127 / 505 / 1009 / 2017 tokens in small and in large
+  // tiles, heads of 128: 38 and 50 / 108 and 102 / 219 and 145 / 469 and 242 us, heads of 64: 27 and 38 / 56 and 74 / 108 and
+  // 106 / 224 and 180 us.
   const int64_t small = (T / p.rows.TB + R) * Hkv * p.rows.NHB;
   p.tall = T > R && T > FEW * p.rows.TB && small * keys(p.rows) >= CROSS / D;
   if (p.tall) {

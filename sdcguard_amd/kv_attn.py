@@ -1,8 +1,9 @@
 """A paged KV cache held in 8 bits: the append that rotates, quantizes and writes a step's keys and values, and the
 attention that reads the cache (no counterpart in the reference, whose checks read caches that others write).
 
-A cache is what KVLedger and the attention check read, (pages, kv heads, slots, 2 head size) with the keys, then the
-values, in the last dimension, here of float8_e4m3fn or int8 codes; scales is (pages, kv heads, 2) fp32: a key is its
+A cache has the layout of a KVLedger's and the attention check's, (pages, kv heads, slots, 2 head size) with the keys, then
+the values, in the last dimension, here of float8_e4m3fn or int8 codes (the ledger takes these, and the scales; the check
+recomputes from 16-bit caches of the queries' type, which kv_append writes too); scales is (pages, kv heads, 2) fp32: a key is its
 code times scales[page, head, 0], a value its code times scales[page, head, 1].  A step is described as the serving
 stack does it: qsl (query_start_loc), seq_lens (lengths with this step's tokens) and bt (block table), int32 on the
 device.  Request r's query tokens qsl[r] .. qsl[r + 1] - 1 are the last positions of its seq_lens[r]; position p is in
