@@ -64,13 +64,24 @@ __device__ __forceinline__ uint32_t scale_field(float v) {
   return e == 0xFFu ? 0u : max(e, (uint32_t)(v != 0.f));
 }
 
-// A query into `row` (of the wave).
-__device__ __forceinline__ void plain_query(const AttendArgs& a, int64_t t, int h, float* row) {
+// A query into `row` (of the wave), after a power of two that brings its largest element under 1, so that no product with codes
+// passes fp32; and the factor on its scores.
+__device__ __forceinline__ float plain_query(const AttendArgs& a, int64_t t, int h, float* row) {
   const uint16_t* q = a.q + t * a.sqt + h * a.sqh;
+  float x[ANY_D / 64], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < ANY_D / 64; ++i) {
+    const int d = (threadIdx.x & 63) + 64 * i;
+    x[i] = d >= a.D ? 0.f : a.fp16 ? half_to_f32<SDC_FP16>(q[d * a.sqd]) : half_to_f32<SDC_BF16>(q[d * a.sqd]);
+    if (fabsf(x[i]) < __builtin_inff()) amax = fmaxf(amax, fabsf(x[i]));
+  }
+  int e = 0;
+  (void)frexpf(wave_max_f32_dpp(amax), &e);
   sdc_wave_lds_fence();                        // (another row's may be read still)
-  for (int d = threadIdx.x & 63; d < a.D; d += 64)
-    row[d] = a.fp16 ? half_to_f32<SDC_FP16>(q[d * a.sqd]) : half_to_f32<SDC_BF16>(q[d * a.sqd]);
+#pragma unroll
+  for (int i = 0; i < ANY_D / 64; ++i) row[(threadIdx.x & 63) + 64 * i] = ldexpf(x[i], -e);
   sdc_wave_lds_fence();
+  return ldexpf(a.scale, e);
 }
 // One query row over keys lo .. hi of request r, by a wave, all in fp32: a lane has a key's score, then elements lane + 64 e of
 // the output, in units of 2^u where values would pass fp32 in their sum.
@@ -79,7 +90,7 @@ struct PlainRow {
   int u;
 };
 template <int CT>
-__device__ __forceinline__ PlainRow plain_row(const AttendArgs& a, const float* q, int r, int hk, int64_t lo, int64_t hi) {
+__device__ __forceinline__ PlainRow plain_row(const AttendArgs& a, const float* q, float scale, int r, int hk, int64_t lo, int64_t hi) {
   const int lane = threadIdx.x & 63, D = a.D;
   PlainRow s{NEG_INF, 0.f, {}, 0};
   for (int64_t b = lo; b < hi; b += 64) {
@@ -95,7 +106,7 @@ __device__ __forceinline__ PlainRow plain_row(const AttendArgs& a, const float* 
       vs = in ? sc[1] : __builtin_nanf("");
       float dot = 0.f;
       for (int d = 0; d < D; ++d) dot = fmaf(q[d], value_of<CT>(a.kv[row + d]), dot);
-      x = dot * ks * a.scale;
+      x = dot * (ks * scale);
     }
     const float mn = fmaxf(s.m, wave_max_f32_dpp(x)), ms = mn == NEG_INF ? 0.f : mn;
     const int u = max(s.u, (int)wave_max_u32_dpp(scale_field(vs)) - 126 - 80);
@@ -138,7 +149,7 @@ __global__ __launch_bounds__(256) void kv_attend_any(AttendArgs a) {
   if (id >= a.st.T * a.Hq) return;
   const int64_t t = id / a.Hq;
   const int h = (int)(id - t * a.Hq);
-  plain_query(a, t, h, qs[w]);
+  const float scale = plain_query(a, t, h, qs[w]);
   Request rq;
   int64_t first;
   const int r = sdc_find_request(a.st, t, 1, 0, rq, first);
@@ -147,7 +158,7 @@ __global__ __launch_bounds__(256) void kv_attend_any(AttendArgs a) {
     hi = min(t - rq.q1 + rq.len + 1, a.maxlen);
     lo = max(t - rq.q1 + rq.len + 1 - a.window, (int64_t)0);
   }
-  write_plain(a, t, h, plain_row<CT>(a, qs[w], r, h / a.G, lo, hi), hi > lo);
+  write_plain(a, t, h, plain_row<CT>(a, qs[w], scale, r, h / a.G, lo, hi), hi > lo);
 }
 
 // ------------------------------------------------------------------------------------------------ few query rows
@@ -348,8 +359,8 @@ __device__ __forceinline__ void plain_part(float* q, int waves) {
     if (tok >= t.ntok || hd >= a.G) continue;
     const int64_t p = t.p0 + tok, token = t.tok0 + tok, lo = max(p - a.window + 1, a0), hi = min(min(p + 1, a.maxlen), a1);
     const int head = t.hk * a.G + hd;
-    plain_query(a, token, head, q);
-    const PlainRow r = plain_row<CT>(a, q, t.r, t.hk, lo, hi);
+    const float scale = plain_query(a, token, head, q);
+    const PlainRow r = plain_row<CT>(a, q, scale, t.r, t.hk, lo, hi);
     if (t.nsp == 1) {
       write_plain(a, token, head, r, hi > lo);
       continue;
@@ -373,6 +384,8 @@ __device__ __forceinline__ void plain_part(float* q, int waves) {
 // 11 bits, in units that put their largest product with a value scale at 2^12 .. 2^15 (scale_exponent).
 // With fp16 outputs that leaves 1.4 times the error of fp32 probabilities against 64 bits; under bf16's own rounding it is gone.
 // Four sequences of 100-131k tokens, 8 heads of 128: 172 us, 5.6 TB/s; 64 of 512-2048 tokens 37 us; one of 500 11 us.
+// Registers for four workgroups a CU where heads are of 64 (24 sequences with a chunk of 500 24.3 us, with three 25.0; 64 decoding
+// 25.5 and 25.1).
 template <int CT, int DP, int PN>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 || PN == 1 ? 2 : 4) void kv_attend_rows(AttendArgs a, Split sp) {
   constexpr int NW = 4, KEYS = 32 * NW;                     // keys that the workgroup's waves take at a time

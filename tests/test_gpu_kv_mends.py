@@ -379,3 +379,17 @@ def test_value_scales_on_both_sides_of_each_limit(N, large):
             c["scales"][::3, :, 1] = 2.0 ** lo
             c["scales"][::7, :, 1] = other
             attend_tight(c)
+
+
+@pytest.mark.parametrize("D,apart", [(40, False), (64, True)])
+@pytest.mark.parametrize("size", [-110, 0, 127])
+def test_plain_rows_take_queries_of_any_size(size, D, apart):
+    """Head sizes that no tile takes, and parts that are left to plain rows, with queries up to bf16's largest and down to small
+    ones: scores of a few units."""
+    c = make(((300, 40), (90, 1)), D=D, Hq=4, Hkv=1, seed=34, garbage=False)
+    c["q"].mul_(2.0 ** (size - 2)).clamp_(-torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).max)
+    c["scales"][..., 0] = 2.0 ** (-size - 6) if size >= 0 else 2.0 ** 104
+    if apart:
+        c["scales"][:, :, 1] = 2.0 ** -70
+        c["scales"][::2, :, 1] = 2.0 ** 40
+    attend_tight(c)
